@@ -22,7 +22,10 @@ INCLUDE = os.path.join(PKG_DIR, "..", "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpropainter_hip.so")
 STAMP_PATH = os.path.join(LIB_DIR, "build_stamp.txt")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result"]
+# packed-fp32-ops off: hipcc otherwise turns ordinary float code into v_pk_{add,mul,fma}_f32, some forms of which have given wrong results
+# now and then; the scalar instructions round alike, so results are unchanged (the host pass warns that it does not know the feature)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 if os.environ.get("PP_DIAG") == "1":       # tuning builds: compiles the diagnostic / ablation kernel variants tools/kbench and
     FLAGS.append("-DPP_DIAG")            # tools/bench_dcn.py select through pp_conv_args_t.impl (never in the shipped library)
 
@@ -61,7 +64,8 @@ def needs_build():
 
 
 def build(force=False, verbose=True):
-    """hipcc --offload-arch=gfx950 -O3 -shared -fPIC; objects are compiled in parallel.  Returns the library path."""
+    """hipcc --offload-arch=gfx950 -O3 -shared -fPIC; objects are compiled in parallel (force: all of them, the object cache is not
+    asked).  Returns the library path."""
     if not force and not needs_build():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -88,7 +92,7 @@ def build(force=False, verbose=True):
                         h.update(f.read())
                     obj = os.path.join(cache, f"{s[:-4]}.{h.hexdigest()[:16]}.o")
                     objs.append(obj)
-                    if os.path.exists(obj):
+                    if os.path.exists(obj) and not force:
                         continue
                     for old in glob.glob(os.path.join(cache, f"{s[:-4]}.*.o")):
                         os.unlink(old)

@@ -7,7 +7,7 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 NAME=$1; shift
 OUT=$R/build/$NAME
 mkdir -p $OUT
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result"
+F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 /opt/rocm/bin/hipcc $F "$@" -c $R/propainter_amd/csrc/conv_gemm_v3.hip -o $OUT/conv_gemm_v3.o 2>/dev/null &
 /opt/rocm/bin/hipcc $F "$@" -c $R/propainter_amd/csrc/conv_gemm_v3s.hip -o $OUT/conv_gemm_v3s.o 2>/dev/null &
 wait

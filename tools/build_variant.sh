@@ -9,7 +9,7 @@ mkdir -p $OUT/obj
 pids=()
 for s in $R/propainter_amd/csrc/*.hip; do
   b=$(basename $s .hip)
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result -DPP_DIAG "$@" -c $s -o $OUT/obj/$b.o &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -DPP_DIAG "$@" -c $s -o $OUT/obj/$b.o &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait $p; done
