@@ -43,6 +43,7 @@ extern "C" {
 #define PP_ACT_SIGMOID 3
 #define PP_ACT_TANH 4
 #define PP_ACT_GELU 5    /* exact erf GELU (torch.nn.GELU default) */
+#define PP_ACT_SILU 6    /* v * sigmoid(v): pp_group_norm and pp_linear_i8 only */
 
 int pp_version(void);
 const char* pp_last_error_string(void);
@@ -439,6 +440,68 @@ int pp_softcomp(const void* tokens, const void* emb_weight, const float* emb_bia
 /* FusionFeedForward's fold -> normalise -> unfold (:82-98) on features [BT, fh*fw, C*49] in the reference order (C = 40):
  * out = unfold(fold(in) / fold(ones)); in != out. */
 int pp_ffn_fold_unfold(const void* in, void* out, int BT, int C, int H, int W, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Group norm, 8-bit token linear layer, attention over a shared prefix
+ * ---------------------------------------------------------------------------------------------- */
+/* GroupNorm + activation over an NHWC map (RAFT/extractor.py:14-18,123-124: norm_fn == 'group'): y = act((x - mean) / sqrt(var + eps) *
+ * gamma + beta), mean / biased variance per image and group of C / groups consecutive channels, gamma / beta fp32 [C] or NULL (1 / 0).
+ * in / out: channel windows [choff, choff + C) of NHWC buffers of dtype (out may be `in` itself, same window); C % 8 == 0, C <= 2048,
+ * groups divides C, strides and offsets multiples of 8, buffers 16-byte aligned.  act: any PP_ACT_* (slope of LRELU = act_param).
+ * Channels of `out` outside its window are left as they are.  stats_ws: caller-owned fp32 workspace of
+ * pp_group_norm_workspace_floats elements, 8-byte aligned.  A NaN or infinity makes its group NaN.  Deterministic. */
+int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, int groups);
+int pp_group_norm(const void* in, int in_cstride, int in_choff, void* out, int out_cstride, int out_choff, const float* gamma,
+                  const float* beta, float* stats_ws, int N, int H, int W, int C, int groups, float eps, int act, float act_param,
+                  int dtype, void* stream);
+
+/* 8-bit codes of token rows: scale[r] = max_k |x[r, k]| / 127 (fp32), q[r, k] = x[r, k] / scale[r] rounded to the nearest integer, ties to
+ * even, of the real quotient.  x: rows of K elements of dtype, x_rstride elements apart (any alignment of dtype; 16-byte aligned rows
+ * are read in 16-byte pieces).  q: int8 rows, q_rstride bytes apart; columns [K, pp_i8_row_bytes(K)) are written as zeros, q and q_rstride
+ * multiples of 16.  A row of zeros has scale 0 and codes 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that a
+ * product with it is NaN.  rows may be 0. */
+int pp_i8_row_bytes(int K);            /* K rounded up to a multiple of 64 (0 < K <= 131072), else PP_ERR_ARG */
+int pp_quantize_tokens(const void* x, int64_t x_rstride, void* q, int64_t q_rstride, float* scale, int64_t rows, int K, int dtype,
+                       void* stream);
+
+/* Linear layer on 8-bit codes: out[m, n] = act(sum_k xq[m, k] * wq[n, k] * xs[m] * ws[n] + bias[n]); the sum is exact (int32).
+ * xq / xs: codes and scales as pp_quantize_tokens writes them (rows of pp_i8_row_bytes(K) bytes, zeros past K, q_rstride bytes apart,
+ * 16-byte aligned).  weight: codes int8 [N, K] (rows wq_rstride bytes apart) laid out once by pp_linear_i8_pack into
+ * pp_linear_i8_weight_bytes(N, K) bytes, 16-byte aligned; ws fp32 [N]; bias fp32 [N] or NULL.  out: rows of out_dtype (PP_F32 / PP_F16),
+ * out_rstride elements apart; columns past N are left as they are.  act: any PP_ACT_*.  M may be 0. */
+int64_t pp_linear_i8_weight_bytes(int N, int K);
+int pp_linear_i8_pack(const void* wq, int64_t wq_rstride, void* weight, int N, int K, void* stream);
+int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out,
+                 int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* stream);
+
+/* Attention of B sequences of Lq query tokens over the keys of a prefix shared by the B / G sequences of a group (sequence b belongs
+ * to group b / (B / G)) and the keys of their own suffix: softmax(scale * q k^T) v in one softmax over both.  The windows of a frame with
+ * their common pooled tokens (model/modules/sparse_transformer.py:205-262) are such a batch, and so are single tokens behind a common
+ * prompt.  Query head h reads key head h / (Hq / Hkv).  Of the prefix the first prefix_lens[g] of P keys count, of the suffix the first
+ * lens[b] of S (values are clamped to [0, P] / [0, S]; what lies behind them is never used, NaN included); with causal = 1 query i sees
+ * suffix keys up to lens[b] - Lq + i (the queries are the last Lq tokens of the sequence).  A query without keys gives zeros.
+ * Strides in elements, multiples of 8 (fp16) / 4 (fp32), the last dimension (D) contiguous, buffers 16-byte aligned; token strides >= D. */
+typedef struct {
+  int32_t dtype;                        /* PP_F16 / PP_F32: q, keys, values, out                   */
+  int32_t B, G, Lq, Hq, Hkv, D, P, S;   /* D 64 or 128; P or S may be 0 (their pointers NULL)      */
+  int32_t causal;
+  float scale;
+  const void* q;  int64_t q_stride[3];          /* [B, Lq, Hq, D]: sequence, token, head            */
+  const void* pk; int64_t pk_stride[3];         /* [G, P, Hkv, D]: group, token, head               */
+  const void* pv; int64_t pv_stride[3];
+  const void* k;  int64_t k_stride[3];          /* [B, S, Hkv, D]                                   */
+  const void* v;  int64_t v_stride[3];
+  void* out;      int64_t out_stride[3];        /* [B, Lq, Hq, D]                                   */
+  const int32_t* prefix_lens;                   /* device [G] or NULL (all P)                       */
+  const int32_t* lens;                          /* device [B] or NULL (all S)                       */
+  void* work;                                   /* device scratch, 16-byte aligned                  */
+  int64_t work_bytes;                           /* >= pp_shared_prefix_attention_workspace_bytes(args)     */
+} pp_prefix_attn_args_t;
+
+int pp_sizeof_prefix_attn_args(void);
+/* scratch of a call with these sizes (0: none needed); pointers, lengths and strides are not looked at */
+int64_t pp_shared_prefix_attention_workspace_bytes(const pp_prefix_attn_args_t* args);
+int pp_shared_prefix_attention(const pp_prefix_attn_args_t* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Diagnostics (tuning tools only: tools/kbench.cpp, tools/bench_attn.py).  Read and clear the in-kernel phase counters of

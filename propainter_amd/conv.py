@@ -372,6 +372,54 @@ class ConvLayer:
         return out
 
 
+ACTS_I8 = {**ACTS, "silu": hip.ACT_SILU}
+
+
+class Int8Linear:
+    """nn.Linear served in 8 bits: weights as int8 codes with one scale per output channel (quantised and laid out once), tokens quantised
+    per row at the call; products are exact integers, scales / bias / activation in fp32 (pp_linear_i8)."""
+
+    def __init__(self, weight, bias=None, device="cuda"):
+        """weight [N, K] (any float dtype), bias [N] or None"""
+        w = weight.detach().to(device=device, dtype=torch.float32).contiguous()
+        hip.require_gpu(w, "Int8Linear")
+        with hip.on_device_of(w):
+            q, s = hip.quantize_tokens(w)
+        self._set(q, s, bias, w.shape[1])
+
+    @classmethod
+    def from_codes(cls, codes, scale, bias=None):
+        """codes int8 [N, K] in [-127, 127] and fp32 scales [N] of a weight that was quantised elsewhere (GPU tensors)"""
+        layer = cls.__new__(cls)
+        layer._set(codes.contiguous(), scale.contiguous(), bias, codes.shape[1])
+        return layer
+
+    def _set(self, codes, scale, bias, K):
+        if scale.shape != (codes.shape[0],) or scale.dtype != torch.float32:
+            raise ValueError(f"Int8Linear: scales must be float32 [{codes.shape[0]}]")
+        if bias is not None and tuple(bias.shape) != (codes.shape[0],):
+            raise ValueError(f"Int8Linear: bias of {tuple(bias.shape)}, {codes.shape[0]} output channels")
+        hip.require_gpu(codes, "Int8Linear")
+        self.K, self.N = int(K), codes.shape[0]
+        with hip.on_device_of(codes):
+            self.weight = hip.linear_i8_pack(codes, self.K)
+        self.scale = scale
+        self.bias = None if bias is None else bias.detach().to(device=codes.device, dtype=torch.float32).contiguous()
+
+    def product(self, codes, scale, act=None, act_param=0.0, out_dtype=torch.float16, out=None):
+        """Tokens as quantize_tokens returned them (several layers may read the same codes) -> [M, N]"""
+        return hip.linear_i8(codes, scale, self.weight, self.scale, self.bias, self.N, self.K, act=ACTS_I8[act], act_param=act_param,
+                             out_dtype=out_dtype, out=out)
+
+    def __call__(self, x, act=None, act_param=0.0, out_dtype=None, out=None):
+        """x [..., K] fp32 / fp16 -> [..., N] (out_dtype: default x's; a given `out` is [rows, >= N] and returned as it is)"""
+        if x.shape[-1] != self.K:
+            raise ValueError(f"Int8Linear: {x.shape[-1]} input channels, built for {self.K}")
+        codes, scale = hip.quantize_tokens(x)
+        y = self.product(codes, scale, act=act, act_param=act_param, out_dtype=out_dtype or x.dtype, out=out)
+        return y if out is not None else y.view(*x.shape[:-1], self.N)
+
+
 _gemm_tables = {}
 
 

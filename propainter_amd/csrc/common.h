@@ -111,6 +111,19 @@ __device__ __forceinline__ float apply_act(float v, int act, float param) {
   return v > 0.f ? v : (act == PP_ACT_RELU ? 0.f : v * slope);
 }
 
+// Activation of the operators that also take PP_ACT_SILU (group norm, 8-bit linear layer); NaN stays NaN.
+__device__ __forceinline__ float act_value(float v, int act, float param) {
+  switch (act) {
+    case PP_ACT_RELU: return v < 0.f ? 0.f : v;
+    case PP_ACT_LRELU: return v < 0.f ? v * param : v;
+    case PP_ACT_SIGMOID: return 1.f / (1.f + __expf(-v));
+    case PP_ACT_TANH: return tanhf(v);
+    case PP_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case PP_ACT_SILU: return v / (1.f + __expf(-v));
+    default: return v;
+  }
+}
+
 // Loads `n` (<= 8) consecutive elements as fp32.
 template <typename T> __device__ __forceinline__ void load8(const T* p, float* v) {
   if constexpr (sizeof(T) == 2) {

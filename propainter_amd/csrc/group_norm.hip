@@ -1,0 +1,204 @@
+// Group norm with an activation over a channels-last map (the norm_fn == 'group' layers of RAFT/extractor.py:14-18,123-124; any C % 8 == 0).
+//
+//   y[n,p,c] = act((x[n,p,c] - mean[n,g]) * rstd[n,g] * gamma[c] + beta[c]),   g = c / (C / groups),
+//   mean and rstd = 1 / sqrt(var + eps) over the H*W pixels and the C / groups channels of a group, var the biased variance.
+//
+// Statistics are held in fp32 as (count, mean, sum of squared deviations) and joined pairwise (Chan et al. 1979): no difference of large
+// sums of squares, so a map whose mean is far from zero loses nothing.  The order of every sum is fixed by the sizes: no atomics.
+#include "common.h"
+
+namespace pp {
+
+struct GnParams {
+  const char* in;
+  char* out;
+  const float* gamma;     // [C] or NULL (1)
+  const float* beta;      // [C] or NULL (0)
+  float* part;            // [N][slices][groups][2] (mean, M2) of a slice
+  long long in_cs, out_cs;
+  int in_co, out_co;
+  int HW, C, groups, cg, slices, ppslice;   // ppslice: pixels per slice
+  float eps, act_param;
+  int act;
+};
+
+__device__ __forceinline__ void chan_merge(float& n, float& m, float& M2, float nb, float mb, float M2b) {
+  if (nb == 0.f) return;
+  const float nt = n + nb, d = mb - m, f = nb / nt;
+  m = fmaf(d, f, m);
+  M2 = M2 + M2b + d * d * (n * f);
+  n = nt;
+}
+
+// 256 threads: column = 8 channels, the rest of the block walks the pixels of one slice.  Sums are taken relative to the slice's first
+// pixel (per channel), so that they hold deviations and not magnitudes.
+template <typename T>
+__global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
+  __shared__ float s1[256 * 8], s2[256 * 8];
+  const int c8 = p.C >> 3, rows = 256 / c8;
+  const int t = threadIdx.x, col = t % c8, pr = t / c8;
+  const bool on = pr < rows;
+  const int slice = blockIdx.x, n = blockIdx.y;
+  const int p0 = slice * p.ppslice;
+  const int np = min(p.ppslice, p.HW - p0);
+  const T* x = reinterpret_cast<const T*>(p.in) + ((long long)n * p.HW + p0) * p.in_cs + p.in_co + col * 8;
+  float shift[8], a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+  if (on) {
+    load8<T>(x, shift);
+    for (int q = pr; q < np; q += rows) {
+      float v[8];
+      load8<T>(x + (long long)q * p.in_cs, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = v[i] - shift[i];
+        a[i] += d;
+        b[i] = fmaf(d, d, b[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { s1[t * 8 + i] = a[i]; s2[t * 8 + i] = b[i]; }
+  for (int h = rows; h > 1;) {                       // rows of the block, halved
+    const int half = (h + 1) >> 1;
+    __syncthreads();
+    if (pr < h - half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s1[t * 8 + i] += s1[(t + half * c8) * 8 + i];
+        s2[t * 8 + i] += s2[(t + half * c8) * 8 + i];
+      }
+    }
+    h = half;
+  }
+  __syncthreads();
+  // per channel (mean, M2), then the channels of each group
+  const T* x0 = reinterpret_cast<const T*>(p.in) + ((long long)n * p.HW + p0) * p.in_cs + p.in_co;
+  for (int c = t; c < p.C; c += 256) {
+    const float m = s1[c] / (float)np;
+    s2[c] = fmaxf(s2[c] - s1[c] * m, s2[c] - s2[c]);      // >= 0; NaN stays NaN
+    s1[c] = to_f32(x0[c]) + m;
+  }
+  __syncthreads();
+  for (int g = t; g < p.groups; g += 256) {
+    float cnt = 0.f, m = 0.f, M2 = 0.f;
+    for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) chan_merge(cnt, m, M2, (float)np, s1[c], s2[c]);
+    float* o = p.part + (((long long)n * p.slices + slice) * p.groups + g) * 2;
+    o[0] = m;
+    o[1] = M2;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
+  __shared__ float gm[2048], gr[2048];                 // mean and rstd of every group (groups <= C <= 2048)
+  __shared__ float part_n[256], part_m[256], part_v[256];
+  const int t = threadIdx.x, n = blockIdx.y;
+  const float* part = p.part + (long long)n * p.slices * p.groups * 2;
+  const int per = p.groups < 256 ? 256 / p.groups : 1;  // threads that share one group's slices
+  for (int g0 = 0; g0 < p.groups; g0 += 256) {
+    const int ng = min(256, p.groups - g0);
+    const int g = t % ng, s0 = t / ng;
+    float cnt = 0.f, m = 0.f, M2 = 0.f;
+    if (s0 < per)
+      for (int s = s0; s < p.slices; s += per) {
+        const int np = min(p.ppslice, p.HW - s * p.ppslice);
+        const float* e = part + ((long long)s * p.groups + g0 + g) * 2;
+        chan_merge(cnt, m, M2, (float)np * (float)p.cg, e[0], e[1]);
+      }
+    part_n[t] = cnt; part_m[t] = m; part_v[t] = M2;
+    for (int h = per; h > 1;) {
+      const int half = (h + 1) >> 1;
+      __syncthreads();
+      if (s0 < h - half) {
+        const int o = t + half * ng;
+        chan_merge(cnt, m, M2, part_n[o], part_m[o], part_v[o]);
+        part_n[t] = cnt; part_m[t] = m; part_v[t] = M2;
+      }
+      h = half;
+    }
+    if (s0 == 0) {
+      gm[g0 + g] = m;
+      gr[g0 + g] = 1.f / sqrtf(M2 / cnt + p.eps);
+    }
+    __syncthreads();
+  }
+  const int c8 = p.C >> 3, rows = 256 / c8, col = t % c8, pr = t / c8;
+  if (pr >= rows) return;
+  float mean[8], mul[8], add[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = col * 8 + i, g = c / p.cg;
+    mean[i] = gm[g];
+    mul[i] = gr[g] * (p.gamma != nullptr ? p.gamma[c] : 1.f);
+    add[i] = p.beta != nullptr ? p.beta[c] : 0.f;
+  }
+  const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + col * 8;
+  T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + col * 8;
+  for (long long q = (long long)blockIdx.x * rows + pr; q < p.HW; q += (long long)gridDim.x * rows) {
+    float v[8];
+    load8<T>(x + q * p.in_cs, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_value(fmaf(v[i] - mean[i], mul[i], add[i]), p.act, p.act_param);
+    store8<T>(y + q * p.out_cs, v);
+  }
+}
+
+}  // namespace pp
+
+using namespace pp;
+
+static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
+  // enough blocks to fill the chip, but no slice under 64 vectors a column set (the joins would cost more than the pixels)
+  const int rows = 256 / (C / 8) > 0 ? 256 / (C / 8) : 1;
+  int want = 1024 / N;
+  if (want < 1) want = 1;
+  int64_t pp = ((int64_t)HW + want - 1) / want;
+  if (pp < 4 * rows) pp = 4 * rows;
+  *ppslice = (int)(pp < HW ? pp : HW);
+  *slices = ceil_div(HW, *ppslice);
+}
+
+extern "C" int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, int groups) {
+  if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 != 0 || C > 2048 || groups <= 0 || C % groups != 0 || (int64_t)H * W > 0x7fffffff) return PP_ERR_ARG;
+  int slices, pps;
+  gn_split(N, H * W, C, &slices, &pps);
+  return (int64_t)N * slices * groups * 2;
+}
+
+extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void* out, int out_cstride, int out_choff, const float* gamma,
+                             const float* beta, float* stats_ws, int N, int H, int W, int C, int groups, float eps, int act, float act_param,
+                             int dtype, void* stream) {
+  PP_REQUIRE(in && out && stats_ws && N > 0 && N <= 65535 && H > 0 && W > 0 && (int64_t)H * W <= 0x7fffffff, PP_ERR_ARG,
+             "pp_group_norm: bad arguments (N=%d H=%d W=%d)", N, H, W);
+  PP_REQUIRE(C > 0 && C % 8 == 0 && C <= 2048 && groups > 0 && C % groups == 0, PP_ERR_ARG,
+             "pp_group_norm: C=%d must be a multiple of 8, <= 2048, and of groups=%d", C, groups);
+  PP_REQUIRE(act >= PP_ACT_NONE && act <= PP_ACT_SILU, PP_ERR_ARG, "pp_group_norm: activation code %d", act);
+  PP_REQUIRE(eps >= 0.f, PP_ERR_ARG, "pp_group_norm: eps must not be negative");
+  PP_REQUIRE(dtype == PP_F32 || dtype == PP_F16, PP_ERR_DTYPE, "pp_group_norm: dtype %d", dtype);
+  PP_REQUIRE(in_choff >= 0 && out_choff >= 0 && in_cstride >= in_choff + C && out_cstride >= out_choff + C, PP_ERR_ARG,
+             "pp_group_norm: channel windows %d+%d of %d, %d+%d of %d", in_choff, C, in_cstride, out_choff, C, out_cstride);
+  PP_REQUIRE((in_cstride | in_choff | out_cstride | out_choff) % 8 == 0 && (uintptr_t)in % 16 == 0 && (uintptr_t)out % 16 == 0 &&
+                 (uintptr_t)stats_ws % 8 == 0,
+             PP_ERR_ALIGN, "pp_group_norm: strides and channel offsets must be multiples of 8, the buffers 16-byte aligned");
+  const int HW = H * W;
+  GnParams p;
+  p.in = (const char*)in; p.out = (char*)out; p.gamma = gamma; p.beta = beta; p.part = stats_ws;
+  p.in_cs = in_cstride; p.out_cs = out_cstride; p.in_co = in_choff; p.out_co = out_choff;
+  p.HW = HW; p.C = C; p.groups = groups; p.cg = C / groups; p.eps = eps; p.act = act; p.act_param = act_param;
+  gn_split(N, HW, C, &p.slices, &p.ppslice);
+  hipStream_t st = (hipStream_t)stream;
+  const int rows = 256 / (C / 8);
+  int blocks = ceil_div(HW, rows);
+  const int most = 2048 / N > 1 ? 2048 / N : 1;
+  if (blocks > most) blocks = most;
+  if (dtype == PP_F16) {
+    hipLaunchKernelGGL((gn_stats_kernel<_Float16>), dim3(p.slices, N), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((gn_apply_kernel<_Float16>), dim3(blocks, N), dim3(256), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((gn_stats_kernel<float>), dim3(p.slices, N), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((gn_apply_kernel<float>), dim3(blocks, N), dim3(256), 0, st, p);
+  }
+  return launch_status("pp_group_norm");
+}

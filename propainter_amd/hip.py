@@ -15,6 +15,7 @@ from . import hazard as _hazard
 
 PP_F32, PP_F16, PP_F16S = 0, 1, 2      # PP_F16S: split-plane fp16 pair (value = hi + lo, lo plane at cstride / 2 in the aux ops)
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = 0, 1, 2, 3, 4, 5
+ACT_SILU = 6        # group_norm and the 8-bit linear layer only
 MAX_SRC = 4
 FUSE_NONE, FUSE_GRU_ZR, FUSE_GRU_H, FUSE_DCN_OFFMASK = 0, 1, 2, 3
 
@@ -60,6 +61,17 @@ class AttnArgs(C.Structure):
     ]
 
 
+class PrefixAttnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("G", C.c_int32), ("Lq", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32),
+        ("D", C.c_int32), ("P", C.c_int32), ("S", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_stride", C.c_int64 * 3), ("pk", C.c_void_p), ("pk_stride", C.c_int64 * 3),
+        ("pv", C.c_void_p), ("pv_stride", C.c_int64 * 3), ("k", C.c_void_p), ("k_stride", C.c_int64 * 3),
+        ("v", C.c_void_p), ("v_stride", C.c_int64 * 3), ("out", C.c_void_p), ("out_stride", C.c_int64 * 3),
+        ("prefix_lens", C.c_void_p), ("lens", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -73,7 +85,10 @@ def lib():
     L.pp_last_error_string.restype = C.c_char_p
     for name in ("pp_conv2d", "pp_sparse_window_attention"):
         getattr(L, name).argtypes = [C.c_void_p, C.c_void_p]
-    if L.pp_sizeof_conv_args() != C.sizeof(ConvArgs) or L.pp_sizeof_attn_args() != C.sizeof(AttnArgs):
+    for name in ("pp_group_norm_workspace_floats", "pp_linear_i8_weight_bytes", "pp_shared_prefix_attention_workspace_bytes"):
+        getattr(L, name).restype = C.c_int64
+    if (L.pp_sizeof_conv_args() != C.sizeof(ConvArgs) or L.pp_sizeof_attn_args() != C.sizeof(AttnArgs) or
+            L.pp_sizeof_prefix_attn_args() != C.sizeof(PrefixAttnArgs)):
         raise RuntimeError("libpropainter_hip.so ABI mismatch with propainter_amd/hip.py (struct sizes differ)")
     _lib = L
     return L
@@ -739,6 +754,157 @@ def instance_norm_split(x, relu=False, eps=1e-5, residual=None, res_choff=0, rel
           lambda: _check(lib().pp_instance_norm_split(_p(x), _pw(out), _pw(ws), _i(N), _i(H), _i(W), _i(Cc), C.c_float(eps), _i(1 if relu else 0),
                                                       _p(residual), _i(residual.shape[-1] if residual is not None else 0), _i(res_choff),
                                                       _i(1 if relu2 else 0), _stream(x)), "pp_instance_norm_split"))
+    return out
+
+
+def _same_device(who, x, *others):
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{who}: tensors on {x.device} and {t.device}")
+
+
+def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, act_param=0.0, out=None, x_choff=0, C_=None, out_choff=0):
+    """GroupNorm + activation over channels [x_choff, x_choff + C_) of x NHWC [N,H,W,Cx] -> channels [out_choff, ..) of `out` (allocated
+    [N,H,W,C_] if None; may be x itself with the same window).  gamma / beta fp32 [C_] or None; act: an ACT_* code (ACT_SILU included),
+    act_param the slope of ACT_LRELU (pp_group_norm)."""
+    N, H, W, Cx = x.shape
+    C_ = Cx - x_choff if C_ is None else C_
+    require_gpu(x, "group_norm")
+    if out is None:
+        out = torch.empty((N, H, W, C_), dtype=x.dtype, device=x.device)
+    _same_device("group_norm", x, gamma, beta, out)
+    assert x.is_contiguous() and out.is_contiguous() and out.dtype == x.dtype and out.shape[:3] == x.shape[:3]
+    for t in (gamma, beta):
+        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.shape == (C_,))
+    if out.data_ptr() == x.data_ptr() and (out.shape != x.shape or out_choff != x_choff):
+        raise ValueError("group_norm: in place needs the same channel window")
+    if N == 0:
+        return out
+    L = lib()
+    n = int(L.pp_group_norm_workspace_floats(_i(N), _i(H), _i(W), _i(C_), _i(groups)))
+    if n < 0:
+        raise ValueError(f"group_norm: map {H}x{W}, {C_} channels (a multiple of 8, at most 2048), {groups} groups (must divide the channels)")
+    ws = torch.empty((n,), dtype=torch.float32, device=x.device)
+    nb = N * H * W * C_ * x.element_size()
+    timed("group_norm", 0, 3 * nb, lambda: _check(L.pp_group_norm(_p(x), _i(Cx), _i(x_choff), _pw(out), _i(out.shape[-1]), _i(out_choff), _p(gamma), _p(beta),
+                                                                  _pw(ws), _i(N), _i(H), _i(W), _i(C_), _i(groups), C.c_float(eps), _i(act),
+                                                                  C.c_float(act_param), _i(dtype_code(x.dtype)), _stream(x)), "pp_group_norm"))
+    return out
+
+
+def i8_row_bytes(K):
+    n = lib().pp_i8_row_bytes(_i(K))
+    if n < 0:
+        raise ValueError(f"8-bit rows hold 1 to 131072 values, not {K}")
+    return n
+
+
+def quantize_tokens(x):
+    """x [..., K] fp32 / fp16, rows any (one) stride apart -> (codes int8 [rows, K padded with zeros to a multiple of 64], scale fp32 [rows]):
+    scale = max|row| / 127, code = row / scale rounded to the nearest integer, ties to even (pp_quantize_tokens).  Rows with a NaN or an
+    infinity: scale NaN."""
+    require_gpu(x, "quantize_tokens")
+    K = x.shape[-1]
+    code = dtype_code(x.dtype)
+    Kp = i8_row_bytes(K)
+    rows = x.numel() // K
+    if K > 1 and x.stride(-1) != 1:
+        raise ValueError("quantize_tokens: the last dimension must be contiguous")
+    x2 = x.view(rows, K) if x.dim() != 2 else x            # (raises where the rows are not one stride apart)
+    q = torch.empty((rows, Kp), dtype=torch.int8, device=x.device)
+    scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    if rows:
+        timed("quantize_tokens", 0, _nbytes(x) + _nbytes(q) + _nbytes(scale),
+              lambda: _check(lib().pp_quantize_tokens(_p(x2), C.c_int64(x2.stride(0) if rows > 1 else Kp), _pw(q), C.c_int64(Kp), _pw(scale), C.c_int64(rows), _i(K),
+                                                      _i(code), _stream(x)), "pp_quantize_tokens"))
+    return q, scale
+
+
+def linear_i8_pack(wq, K=None):
+    """Codes int8 [N, >= K] -> the weight layout of linear_i8 (pp_linear_i8_pack)."""
+    require_gpu(wq, "linear_i8_pack")
+    N = wq.shape[0]
+    K = wq.shape[1] if K is None else K
+    assert wq.dtype == torch.int8 and wq.dim() == 2 and wq.is_contiguous() and wq.shape[1] >= K
+    n = int(lib().pp_linear_i8_weight_bytes(_i(N), _i(K)))
+    if n < 0:
+        raise ValueError(f"8-bit linear layer of {K} inputs and {N} outputs: 1 to 131072 inputs and 1 to 4194240 outputs")
+    w = torch.empty((n,), dtype=torch.int8, device=wq.device)
+    _check(lib().pp_linear_i8_pack(_p(wq), C.c_int64(wq.shape[1]), _pw(w), _i(N), _i(K), _stream(wq)), "pp_linear_i8_pack")
+    return w
+
+
+def linear_i8(q, scale, weight, wscale, bias, N, K, act=ACT_NONE, act_param=0.0, out_dtype=torch.float16, out=None):
+    """act(codes @ weight codes^T * scale * wscale + bias): q int8 [M, i8_row_bytes(K)], scale fp32 [M] (quantize_tokens), weight from
+    linear_i8_pack, wscale / bias fp32 [N] -> out [M, N] of out_dtype (or the first N columns of a given `out` [M, >= N])."""
+    require_gpu(q, "linear_i8")
+    M = q.shape[0]
+    if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous() or q.shape[1] != i8_row_bytes(K):
+        raise ValueError(f"linear_i8: codes must be int8 [M, {i8_row_bytes(K)}] as quantize_tokens returns them, got {q.dtype} {tuple(q.shape)}")
+    if scale.shape != (M,) or scale.dtype != torch.float32 or not scale.is_contiguous():
+        raise ValueError(f"linear_i8: scales must be float32 [{M}]")
+    for t in (wscale, bias):
+        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.shape == (N,))
+    assert weight.numel() == int(lib().pp_linear_i8_weight_bytes(_i(N), _i(K))) and weight.dtype == torch.int8 and weight.is_contiguous()
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=q.device)
+    if out.dim() != 2 or out.shape[0] != M or out.shape[1] < N or (M and out.stride(1) != 1):
+        raise ValueError(f"linear_i8: out must be [{M}, >= {N}] with contiguous rows")
+    _same_device("linear_i8", q, scale, weight, wscale, bias, out)
+    code = dtype_code(out.dtype)
+    if M:
+        timed("linear_i8", 2.0 * M * N * K, _nbytes(q) + _nbytes(weight) + M * N * out.element_size(),
+              lambda: _check(lib().pp_linear_i8(_p(q), C.c_int64(q.shape[1]), _p(scale), _p(weight), _p(wscale), _p(bias), _pw(out), C.c_int64(max(out.stride(0), N)),
+                                                C.c_int64(M), _i(N), _i(K), _i(act), C.c_float(act_param), _i(code), _stream(q)), "pp_linear_i8"))
+    return out
+
+
+def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal=False, scale=None, out=None):
+    """softmax(scale * q K^T) V per sequence over the keys of a prefix that the B / G sequences of a group share and their own suffix keys:
+    q [B,Lq,Hq,D]; pk / pv [G,P,Hkv,D] or None; k / v [B,S,Hkv,D] or None; Hq a multiple of Hkv, D 64 or 128, fp16 or fp32, any strides with a
+    contiguous last dimension.  Sequence b belongs to group b // (B // G).  prefix_lens int32 [G] / lens int32 [B] (device): the keys that
+    count (default: all); causal: query i sees suffix keys up to lens[b] - Lq + i.  scale: default 1 / sqrt(D).  A query without keys gives
+    zeros.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
+    require_gpu(q, "shared_prefix_attention")
+    B, Lq, Hq, D = q.shape
+    if (pk is None) != (pv is None) or (k is None) != (v is None):
+        raise ValueError("shared_prefix_attention: keys and values come together")
+    a = PrefixAttnArgs()
+    a.dtype, a.B, a.Lq, a.Hq, a.D = dtype_code(q.dtype), B, Lq, Hq, D
+    a.G, a.P = (pk.shape[0], pk.shape[1]) if pk is not None else (1, 0)
+    a.S = k.shape[1] if k is not None else 0
+    a.Hkv = pk.shape[2] if pk is not None else (k.shape[2] if k is not None else Hq)
+    if out is None:
+        out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    _same_device("shared_prefix_attention", q, pk, pv, k, v, prefix_lens, lens, out)
+    for name, t, shape in (("q", q, (B, Lq, Hq, D)), ("pk", pk, (a.G, a.P, a.Hkv, D)), ("pv", pv, (a.G, a.P, a.Hkv, D)), ("k", k, (B, a.S, a.Hkv, D)),
+                           ("v", v, (B, a.S, a.Hkv, D)), ("out", out, (B, Lq, Hq, D))):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape or t.dtype != q.dtype or (t.numel() and t.stride(3) != 1):
+            raise ValueError(f"shared_prefix_attention: {name} is {t.dtype} {tuple(t.shape)}, expected {q.dtype} {shape} with a contiguous last dimension")
+        setattr(a, name, t.data_ptr())
+        getattr(a, name + "_stride")[:] = t.stride()[:3]
+    for name, t, n in (("prefix_lens", prefix_lens, a.G), ("lens", lens, B)):
+        if t is not None:
+            if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+                raise ValueError(f"shared_prefix_attention: {name} must be int32 [{n}]")
+            setattr(a, name, t.data_ptr())
+    a.causal, a.scale = int(bool(causal)), float(scale) if scale is not None else D ** -0.5
+    need = int(lib().pp_shared_prefix_attention_workspace_bytes(C.byref(a)))
+    if need < 0:
+        _check(need, "pp_shared_prefix_attention")
+    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+    if work is not None:
+        a.work, a.work_bytes = work.data_ptr(), need
+    for t in (q, pk, pv, k, v, prefix_lens, lens):
+        _p(t)
+    for t in (out, work):
+        _pw(t)
+    esz = q.element_size()
+    nb = esz * D * (2 * B * Lq * Hq + 2 * a.Hkv * (a.G * a.P + B * a.S))
+    timed("shared_prefix_attention", 4.0 * D * Hq * B * Lq * (a.P + a.S), nb,
+          lambda: _check(lib().pp_shared_prefix_attention(C.byref(a), _stream(q)), "pp_shared_prefix_attention"))
     return out
 
 
