@@ -3,67 +3,473 @@
 //   out[b,i,h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q[b,i,h] . k_j - m),   m = max_j
 //   j over prefix_lens[g] shared keys of group g = b / (B / G), then over lens[b] (causal: the first lens[b] - Lq + i + 1) own keys
 //
-// One wave per (query, head): the kernel every other form is checked against.  fp32 arithmetic, online maximum and sum.
+// Rows.  The queries that read one key head form rows: Lq * rep of a sequence (rep = Hq / Hkv query heads a key head), or, packed, those of
+// ALL sequences of a group, which is how a prefix is read once for the whole batch.  A part of the work is a set of row spaces with the keys
+// they walk; a call is one part (every sequence walks prefix and suffix) or two (packed rows walk the prefix, single sequences their
+// suffix).  Where a row's keys are split over several blocks, each leaves (max, sum, unnormalised output) in fp32 scratch and
+// pa_join_kernel joins them in a fixed order.
+//
+// pa_tile_kernel: 4 waves, key tiles in LDS (K swizzled, V skewed), the next tile's global loads in flight during the products.
+//   S^T = K Q^T and O^T += V^T P^T on 16x16 MFMA tiles: a lane holds scores of ONE query (column l & 15), so the row maximum takes two
+//   lane swaps, and its scores are the second product's operand as they are, keys relabelled.
+//   WK = false: a wave owns 16 QT rows and every key of a tile (many rows).  WK = true: the four waves share 16 QT rows and take a quarter
+//   of a tile's keys each, joined through LDS at the end (few rows: single tokens).
 #include "common.h"
+#include "attn_lanes.h"
 
 namespace pp {
 
+struct PaPart {
+  int nper;              // sequences a row space packs (1 or nseq)
+  int rows, rowblocks;   // rows of a space, blocks that cover them
+  int prefix, suffix;    // keys it walks
+  int nsplit, slot0;     // key splits; first scratch slot
+};
 struct PaParams {
   const char *q, *pk, *pv, *k, *v;
   char* out;
   const int *plens, *lens;
+  float* part_o;         // [slots][B * Lq * Hq][D], NULL: one split writes the output itself
+  float* part_ml;        // [slots][B * Lq * Hq][2]
   long long qs[3], pks[3], pvs[3], ks[3], vs[3], os[3];
-  int B, G, nseq, Lq, Hq, Hkv, rep, P, S, causal;
-  float sc2;      // scale * log2(e)
+  int B, G, nseq, Lq, Hq, Hkv, rep, P, S, causal, slots;
+  float sc2;             // |scale| * log2(e)  (1 if scale is 0)
+  float qsign;           // sign of scale (0 if it is 0), taken into the queries
+  PaPart part;
 };
+
+constexpr float PA_NONE = -3.4028235e38f;   // running maximum before the first key: finite, so that masked scores (-inf) weigh 0
 
 __device__ __forceinline__ int clamp_len(const int* lens, int i, int most) {
   const int n = lens != nullptr ? lens[i] : most;
   return n < 0 ? 0 : (n > most ? most : n);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void pa_simple_kernel(const PaParams p) {
-  const int lane = threadIdx.x & 63;
-  const long long id = blockIdx.x * 4ll + (threadIdx.x >> 6);
-  if (id >= (long long)p.B * p.Lq * p.Hq) return;
-  const int h = (int)(id % p.Hq);
-  const int i = (int)(id / p.Hq % p.Lq);
-  const int b = (int)(id / ((long long)p.Hq * p.Lq));
-  const int g = b / p.nseq, hk = h / p.rep;
-  constexpr int E = D / 64;
-  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] + lane;
-  float qv[E], acc[E];
+#if defined(__HIP_DEVICE_COMPILE__)
+template <typename T> struct PaOps;
+template <> struct PaOps<_Float16> {
+  typedef f16x8 frag;      // 16 bytes of a row: 8 consecutive channels
+  static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct PaOps<float> {
+  typedef f32x4 frag;      // 16 bytes of a row: 4 consecutive channels, one contraction slot of 4 products
+  static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) { qv[e] = to_f32(q[e * 64]) * p.sc2; acc[e] = 0.f; }
-  const int np = clamp_len(p.plens, g, p.P);
-  int ns = clamp_len(p.lens, b, p.S);
-  if (p.causal) ns = max(0, min(ns, ns - p.Lq + i + 1));
-  float m = -3.4028235e38f, l = 0.f;
-  for (int j = 0; j < np + ns; ++j) {
-    const T *kr, *vr;
-    if (j < np) {
-      kr = reinterpret_cast<const T*>(p.pk) + g * p.pks[0] + j * p.pks[1] + hk * p.pks[2] + lane;
-      vr = reinterpret_cast<const T*>(p.pv) + g * p.pvs[0] + j * p.pvs[1] + hk * p.pvs[2] + lane;
-    } else {
-      kr = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + (j - np) * p.ks[1] + hk * p.ks[2] + lane;
-      vr = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + (j - np) * p.vs[1] + hk * p.vs[2] + lane;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(qv[e], to_f32(kr[e * 64]), s);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    const float mn = fmaxf(m, s);
-    const float alpha = __builtin_amdgcn_exp2f(m - mn), pe = __builtin_amdgcn_exp2f(s - mn);
-    l = l * alpha + pe;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(pe, to_f32(vr[e * 64]), acc[e] * alpha);
-    m = mn;
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
   }
-  T* o = reinterpret_cast<T*>(p.out) + b * p.os[0] + i * p.os[1] + h * p.os[2] + lane;
+};
+#endif
+
+template <typename T, int D, bool WK> struct PaTile {
+  static constexpr bool F16 = sizeof(T) == 2;
+  static constexpr int KT = F16 && WK ? 128 : 64;             // keys of a tile
+  static constexpr int NK = WK ? KT / 64 : 4;                 // 16-key tiles of a wave
+  static constexpr int SLOTS = D * (int)sizeof(T) / 16;       // 16-byte slots of a key row
+  static constexpr int STEPS = SLOTS / 4;                     // fragments of a row
+  static constexpr int VLD = F16 ? D + 4 : D + 16;            // V row stride (elements): skews the banks of a column's keys
+  static constexpr int LOADS = KT * SLOTS / 256;              // 16-byte pieces a thread stages of K and of V
+  static constexpr int KBYTES = KT * D * (int)sizeof(T), VBYTES = KT * VLD * (int)sizeof(T);
+};
+
+template <typename T, int D, int QT, bool WK>
+__global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef PaTile<T, D, WK> C;
+  typedef typename PaOps<T>::frag frag;
+  constexpr int KT = C::KT, NK = C::NK, STEPS = C::STEPS, DT = D / 16;
+  constexpr int JOIN = WK ? 4 * 16 * QT * (D + 4) * 4 : 0;
+  constexpr int LDS = C::KBYTES + C::VBYTES > JOIN ? C::KBYTES + C::VBYTES : JOIN;
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
+  __shared__ float wave_ml[WK ? 4 * 16 * QT * 2 : 1];
+  T* Ks = reinterpret_cast<T*>(lds);
+  T* Vs = reinterpret_cast<T*>(lds + C::KBYTES);
+  const PaPart& pt = p.part;
+
+  // ---- block -> (row block fastest, split, key head, row space); blocks 8 apart share an XCD: each XCD gets one contiguous run, so that
+  // the row blocks that read the same keys meet in one L2
+  long long id = blockIdx.x;
+  {
+    const long long n = gridDim.x, per = n >> 3, extra = n & 7, x = id & 7;
+    id = x * per + (x < extra ? x : extra) + (id >> 3);
+  }
+  const int rb = (int)(id % pt.rowblocks); id /= pt.rowblocks;
+  const int split = (int)(id % pt.nsplit); id /= pt.nsplit;
+  const int hk = (int)(id % p.Hkv);
+  const int space = (int)(id / p.Hkv);
+  const int b0 = space * pt.nper, g = b0 / p.nseq;
+  const int rpseq = p.Lq * p.rep;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lg = lane >> 4, lc = lane & 15;
+  const int row0 = rb * 16 * QT * (WK ? 1 : 4);
+  const int row_end = min(pt.rows, row0 + 16 * QT * (WK ? 1 : 4));
+
+  const int np = pt.prefix ? clamp_len(p.plens, g, p.P) : 0;
+  const int ns = pt.suffix ? clamp_len(p.lens, b0, p.S) : 0;
+  int vis_min = ns, vis_max = ns;                 // suffix keys the block's first / last row sees
+  if (pt.suffix && p.causal) {
+    vis_min = min(ns, max(0, ns - p.Lq + row0 / p.rep + 1));
+    vis_max = min(ns, max(0, ns - p.Lq + (row_end - 1) / p.rep + 1));
+  }
+  const int ptiles = (np + KT - 1) / KT;
+  const int tiles = ptiles + (vis_max + KT - 1) / KT;
+  const int t0 = (int)((long long)tiles * split / pt.nsplit), t1 = (int)((long long)tiles * (split + 1) / pt.nsplit);
+
+  // ---- this lane's queries (column lane & 15 of the wave's row tiles)
+  frag qf[QT][STEPS];
+  long long rowid[QT];
+  int vis[QT];
+  char* optr[QT];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e * 64] = from_f32<T>(np + ns > 0 ? acc[e] / l : 0.f);
+  for (int qt = 0; qt < QT; ++qt) {
+    const int r = row0 + (WK ? qt : wave * QT + qt) * 16 + lc;
+    const bool ok = r < pt.rows;
+    const int rr = ok ? r : 0;
+    const int sq = rr / rpseq, rest = rr - sq * rpseq;
+    const int i = rest / p.rep, h = hk * p.rep + (rest - i * p.rep);
+    const int b = b0 + sq;
+    rowid[qt] = ok ? ((long long)b * p.Lq + i) * p.Hq + h : -1;
+    vis[qt] = p.causal ? max(0, ns - p.Lq + i + 1) : ns;
+    optr[qt] = p.out + (b * p.os[0] + i * p.os[1] + h * p.os[2]) * (long long)sizeof(T);
+    const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      frag f = *reinterpret_cast<const frag*>(qp + (s * 4 + lg) * (16 / sizeof(T)));
+      if (p.qsign != 1.f) f *= (T)p.qsign;
+      qf[qt][s] = f;
+    }
+  }
+
+  f32x4 oacc[QT][DT];
+  float m_run[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = PA_NONE;
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ---- staging: a tile's valid keys lie inside the buffer descriptor built for it, the rest comes back as zeros (so that nothing behind a
+  // length is used); 64-bit base per tile, 32-bit offsets inside it
+  u32x4 kr[C::LOADS], vr[C::LOADS];
+  auto tile_keys = [&](int t) {                    // valid keys of tile t
+    return t < ptiles ? min(KT, np - t * KT) : min(KT, vis_max - (t - ptiles) * KT);
+  };
+  auto load_tile = [&](int t) {
+    const bool pre = t < ptiles;
+    const long long j0 = (long long)(pre ? t : t - ptiles) * KT;
+    const long long kts = pre ? p.pks[1] : p.ks[1], vts = pre ? p.pvs[1] : p.vs[1];
+    const T* kb = pre ? reinterpret_cast<const T*>(p.pk) + g * p.pks[0] + hk * p.pks[2] : reinterpret_cast<const T*>(p.k) + b0 * p.ks[0] + hk * p.ks[2];
+    const T* vb = pre ? reinterpret_cast<const T*>(p.pv) + g * p.pvs[0] + hk * p.pvs[2] : reinterpret_cast<const T*>(p.v) + b0 * p.vs[0] + hk * p.vs[2];
+    const unsigned kp = (unsigned)kts * sizeof(T), vp = (unsigned)vts * sizeof(T);
+    const int n = tile_keys(t);
+    const __amdgpu_buffer_rsrc_t rk = uniform_buffer_rsrc(kb + j0 * kts, (int)((n - 1) * kp + D * sizeof(T)));
+    const __amdgpu_buffer_rsrc_t rv = uniform_buffer_rsrc(vb + j0 * vts, (int)((n - 1) * vp + D * sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < C::LOADS; ++i) {
+      const int c = tid + 256 * i, key = c / C::SLOTS, sl = c % C::SLOTS;
+      kr[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(key < n ? key * kp + sl * 16 : 0xfffffff0u), 0, 0);
+      vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(key < n ? key * vp + sl * 16 : 0xfffffff0u), 0, 0);
+    }
+  };
+  auto swz = [](int key) { return C::SLOTS >= 16 ? key & 15 : (key >> 1) & 7; };
+  auto store_tile = [&]() {
+#pragma unroll
+    for (int i = 0; i < C::LOADS; ++i) {
+      const int c = tid + 256 * i, key = c / C::SLOTS, sl = c % C::SLOTS;
+      *reinterpret_cast<u32x4*>(&Ks[key * D + (sl ^ swz(key)) * (16 / sizeof(T))]) = kr[i];
+      T* vrow = &Vs[key * C::VLD + sl * (16 / sizeof(T))];
+      if constexpr (C::F16) {                      // rows are 8-byte aligned: two halves, in opposite order in the two halves of a row
+        const int sel = sl >= C::SLOTS / 2;
+        const u32x2 lo = {vr[i][0], vr[i][1]}, hi = {vr[i][2], vr[i][3]};
+        *reinterpret_cast<u32x2*>(vrow + sel * 4) = sel ? hi : lo;
+        *reinterpret_cast<u32x2*>(vrow + (sel ^ 1) * 4) = sel ? lo : hi;
+      } else {
+        *reinterpret_cast<u32x4*>(vrow) = vr[i];
+      }
+    }
+  };
+
+  const int wkey = WK ? wave * NK * 16 : 0;        // first key of the wave inside a tile
+  if (t0 < t1) load_tile(t0);
+  for (int t = t0; t < t1; ++t) {
+    store_tile();
+    __syncthreads();
+    if (t + 1 < t1) load_tile(t + 1);
+    // ---- scores: sacc[qt][kt][r] = key wkey + kt * 16 + lg * 4 + r, query lc of row tile qt
+    f32x4 sacc[QT][NK];
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int key = wkey + kt * 16 + lc;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const frag kf = *reinterpret_cast<const frag*>(&Ks[key * D + ((s * 4 + lg) ^ swz(key)) * (16 / sizeof(T))]);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = PaOps<T>::mfma(kf, qf[qt][s], sacc[qt][kt]);
+      }
+    }
+    // ---- online softmax in the exp2 domain
+    const int n = tile_keys(t), j0 = (t - ptiles) * KT;
+    const bool cut = p.causal && t >= ptiles && j0 + n > vis_min;      // rows of the block see different parts of the tile
+    constexpr int NP = C::F16 ? (NK + 1) / 2 : 1;
+    f16x8 pfr[QT][NP];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if (n < KT || cut) {
+        const int most = cut ? min(n, vis[qt] - j0) : n;
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (wkey + kt * 16 + lg * 4 + r >= most) sacc[qt][kt][r] = -INFINITY;
+      }
+      float tmax = sacc[qt][0][0];
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
+      tmax = rows_max(tmax);
+      const float m_new = fmaxf(m_run[qt], tmax * p.sc2);
+      const bool moved = m_new > m_run[qt];
+      float psum = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, -m_new));
+          psum += e;
+          if constexpr (C::F16) pfr[qt][kt >> 1][(kt & 1) * 4 + r] = (_Float16)e;    // weights in the values' type: the product's operand
+          else sacc[qt][kt][r] = e;
+        }
+      if (__builtin_amdgcn_ballot_w64(moved) != 0ull) {
+        const float alpha = __builtin_amdgcn_exp2f(m_run[qt] - m_new);
+        l_run[qt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oacc[qt][d] *= alpha;
+      }
+      m_run[qt] = m_new;
+      l_run[qt] += psum;                           // this lane's keys; the four lane groups are summed at the end
+    }
+    // ---- O^T += V^T P^T
+    if constexpr (C::F16) {
+      // contraction slot lg * 8 + e of a 32-key step is key (e >> 2) * 16 + lg * 4 + (e & 3); accumulator row i of tile d is channel
+      // (i / 4) * (D / 4) + d * 4 + i % 4: a lane ends with D / 4 consecutive channels of its query
+      const _Float16* vb = reinterpret_cast<const _Float16*>(Vs) + (wkey + lg * 4 + (lc >> 2)) * C::VLD + (lane & 3) * (D / 4);
+#pragma unroll
+      for (int j = 0; j < NK / 2; ++j)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const f16x4 v0 = lds_read_tr16(vb + 32 * j * C::VLD + d * 4);
+          const f16x4 v1 = lds_read_tr16(vb + (32 * j + 16) * C::VLD + d * 4);
+          const f16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pfr[qt][j], oacc[qt][d], 0, 0, 0);
+        }
+    } else {
+      // one key a lane group: slot lg is key kt * 16 + lg * 4 + r; accumulator row i of tile d is channel d * 16 + i
+      const float* vb = reinterpret_cast<const float*>(Vs) + (wkey + lg * 4) * C::VLD + lc;
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const float vv = vb[(kt * 16 + r) * C::VLD + d * 16];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, sacc[qt][kt][r], oacc[qt][d], 0, 0, 0);
+          }
+    }
+    __syncthreads();
+  }
+
+  // channel of accumulator element (d, r) of this lane
+  auto chan = [&](int d, int r) { return C::F16 ? lg * (D / 4) + d * 4 + r : d * 16 + lg * 4 + r; };
+  if constexpr (!WK) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float l = rows_sum(l_run[qt]);
+      if (rowid[qt] < 0) continue;
+      if (p.part_o != nullptr) {
+        const long long at = (pt.slot0 + split) * ((long long)p.B * p.Lq * p.Hq) + rowid[qt];
+        if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_run[qt], l);
+        if (t0 < t1) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + chan(d, 0)) = oacc[qt][d];
+        }
+      } else {
+        const float inv = l != 0.f ? 1.f / l : 0.f;           // no keys: zeros
+        T* o = reinterpret_cast<T*>(optr[qt]);
+        if constexpr (C::F16) {
+#pragma unroll
+          for (int d = 0; d < DT; d += 2) {
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) { v[r] = oacc[qt][d][r] * inv; v[4 + r] = oacc[qt][d + 1][r] * inv; }
+            store8<T>(o + chan(d, 0), v);
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + chan(d, 0)) = oacc[qt][d] * inv;
+        }
+      }
+    }
+  } else {
+    // join the four waves: every wave scales its rows to the common maximum, LDS holds [wave][row][D + 4] floats
+    float* jo = reinterpret_cast<float*>(lds);
+    constexpr int JLD = D + 4;
+    float l[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      l[qt] = rows_sum(l_run[qt]);
+      if (lg == 0) {
+        wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2] = m_run[qt];
+        wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2 + 1] = l[qt];
+      }
+    }
+    __syncthreads();
+    float mj[QT], lj[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float* e = wave_ml + (qt * 16 + lc) * 2;
+      constexpr int W = 16 * QT * 2;
+      mj[qt] = fmaxf(fmaxf(e[0], e[W]), fmaxf(e[2 * W], e[3 * W]));
+      lj[qt] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) lj[qt] += e[w * W + 1] * __builtin_amdgcn_exp2f(e[w * W] - mj[qt]);
+      const float f = __builtin_amdgcn_exp2f(m_run[qt] - mj[qt]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + chan(d, 0)) = oacc[qt][d] * f;
+    }
+    __syncthreads();
+    // wave w finishes rows lc of its quarter of the channels: lane -> row lc, channels wave * D / 4 + lg * D / 16 ..
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if (rowid[qt] < 0) continue;
+      const int c0 = wave * (D / 4) + lg * (D / 16);
+      const float* e = jo + (qt * 16 + lc) * JLD + c0;
+      constexpr int W = 16 * QT * JLD;
+      const float inv = lj[qt] != 0.f ? 1.f / lj[qt] : 0.f;
+      const long long at = (pt.slot0 + split) * ((long long)p.B * p.Lq * p.Hq) + rowid[qt];
+      if (p.part_o != nullptr && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 4) {
+        f32x4 v = *reinterpret_cast<const f32x4*>(e + c);
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + c);
+        if (p.part_o != nullptr) {
+          if (t0 < t1) *reinterpret_cast<f32x4*>(p.part_o + at * D + c0 + c) = v;
+        } else if constexpr (C::F16) {
+          const f16x4 o = {(_Float16)(v[0] * inv), (_Float16)(v[1] * inv), (_Float16)(v[2] * inv), (_Float16)(v[3] * inv)};
+          *reinterpret_cast<f16x4*>(reinterpret_cast<T*>(optr[qt]) + c0 + c) = o;
+        } else {
+          *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(optr[qt]) + c0 + c) = v * inv;
+        }
+      }
+    }
+  }
+#endif
+}
+
+// One wave per row: the slots' outputs, weighted by exp2(max - common max), over the weighted sum.  A slot without keys (sum 0) left no output.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p) {
+  const int lane = threadIdx.x & 63;
+  const long long rows = (long long)p.B * p.Lq * p.Hq;
+  const long long row = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  constexpr int E = D / 64;
+  float m = PA_NONE, l = 0.f;                      // slots <= 64: one a lane
+  if (lane < p.slots) {
+    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + (lane * rows + row) * 2);
+    m = e.x;
+    l = e.y;
+  }
+  float mj = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mj = fmaxf(mj, __shfl_xor(mj, o));
+  const float w = l != 0.f ? __builtin_amdgcn_exp2f(m - mj) : 0.f;
+  float total = l * w;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < p.slots; ++s) {
+    const float ls = __shfl(l, s), ws = __shfl(w, s);
+    if (ls != 0.f) {                               // (a NaN sum is not 0: its output is read and stays NaN)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p.part_o[(s * rows + row) * D + lane * E + e], acc[e]);
+    }
+  }
+  const int h = (int)(row % p.Hq), i = (int)(row / p.Hq % p.Lq), b = (int)(row / p.Hq / p.Lq);
+  T* o = reinterpret_cast<T*>(p.out) + b * p.os[0] + i * p.os[1] + h * p.os[2] + lane * E;
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
+}
+
+// ---- the plan of a call: which parts, which tile form, how many key splits.  A function of sizes and types alone (lengths stay on the device).
+struct PaPlan {
+  int nparts, slots;
+  PaPart part[2];
+  int qt[2], wk[2];
+  long long blocks[2];
+};
+
+inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
+  PaPlan r{};
+  const int nseq = a->B / a->G, rep = a->Hq / a->Hkv;
+  const long long R = (long long)a->Lq * rep;
+  const bool packed = a->P > 0 && nseq > 1 && R <= 32;
+  auto add = [&](int nper, int prefix, int suffix) {
+    PaPart& t = r.part[r.nparts];
+    t.nper = nper; t.prefix = prefix; t.suffix = suffix;
+    t.rows = (int)(R * nper);
+    int& qt = r.qt[r.nparts];
+    int& wk = r.wk[r.nparts];
+    wk = t.rows <= 32;
+    qt = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 ? 1 : 2;
+    const int per = 16 * qt * (wk ? 1 : 4);
+    t.rowblocks = ceil_div(t.rows, per);
+    const long long blocks = (long long)(a->B / nper) * a->Hkv * t.rowblocks;
+    const int kt = a->dtype == PP_F16 && wk ? 128 : 64;
+    const int tiles = (prefix ? ceil_div(a->P, kt) : 0) + (suffix ? ceil_div(a->S, kt) : 0);
+    long long n = blocks > 0 ? 512 / blocks : 1;
+    if (n > tiles / 2) n = tiles / 2;
+    if (n > 32) n = 32;
+    if (n < 1) n = 1;
+    t.nsplit = (int)n;
+    t.slot0 = r.slots;
+    r.slots += t.nsplit;
+    r.blocks[r.nparts] = blocks * n;
+    ++r.nparts;
+  };
+  if (packed) {
+    add(nseq, 1, 0);
+    if (a->S > 0) add(1, 0, 1);
+  } else {
+    add(1, a->P > 0, a->S > 0);
+  }
+  return r;
+}
+
+template <typename T, int D>
+static void pa_launch(const PaPlan& plan, PaParams p, hipStream_t st) {
+  for (int i = 0; i < plan.nparts; ++i) {
+    p.part = plan.part[i];
+    const dim3 grid((unsigned)plan.blocks[i]), block(256);
+    if (plan.wk[i]) {
+      if (plan.qt[i] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, true>), grid, block, 0, st, p);
+      else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, true>), grid, block, 0, st, p);
+    } else {
+      if (plan.qt[i] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, false>), grid, block, 0, st, p);
+      else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, false>), grid, block, 0, st, p);
+    }
+  }
+  if (plan.slots > 1)
+    hipLaunchKernelGGL((pa_join_kernel<T, D>), dim3((unsigned)(((long long)p.B * p.Lq * p.Hq + 3) / 4)), dim3(256), 0, st, p);
 }
 
 }  // namespace pp
@@ -85,7 +491,10 @@ static int pa_check_sizes(const pp_prefix_attn_args_t* a) {
 
 extern "C" int64_t pp_shared_prefix_attention_workspace_bytes(const pp_prefix_attn_args_t* a) {
   const int rc = pa_check_sizes(a);
-  return rc != 0 ? rc : 0;
+  if (rc != 0) return rc;
+  if (a->B == 0 || a->Lq == 0) return 0;
+  const PaPlan plan = pa_plan(a);
+  return plan.slots > 1 ? (int64_t)plan.slots * a->B * a->Lq * a->Hq * (a->D + 2) * 4 : 0;
 }
 
 static int pa_check_tensor(const char* name, const void* ptr, const int64_t* st, int n0, int n1, int n2, int D, int dtype) {
@@ -131,13 +540,20 @@ extern "C" int pp_shared_prefix_attention(const pp_prefix_attn_args_t* a, void* 
     for (int i = 0; i < 3; ++i) to[t][i] = from[t][i];
   p.B = a->B; p.G = a->G; p.nseq = a->B / a->G; p.Lq = a->Lq; p.Hq = a->Hq; p.Hkv = a->Hkv; p.rep = a->Hq / a->Hkv; p.P = a->P; p.S = a->S;
   p.causal = a->causal;
-  p.sc2 = a->scale * 1.4426950408889634f;
+  p.sc2 = a->scale != 0.f ? fabsf(a->scale) * 1.4426950408889634f : 1.f;
+  p.qsign = a->scale > 0.f ? 1.f : a->scale < 0.f ? -1.f : 0.f;
+  const PaPlan plan = pa_plan(a);
+  PP_REQUIRE(plan.blocks[0] <= (1 << 23) && plan.blocks[1] <= (1 << 23), PP_ERR_ARG, "pp_shared_prefix_attention: too many blocks of work");
+  p.slots = plan.slots;
+  p.part_o = plan.slots > 1 ? (float*)a->work : nullptr;
+  p.part_ml = plan.slots > 1 ? (float*)a->work + (int64_t)plan.slots * a->B * a->Lq * a->Hq * a->D : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(((long long)a->B * a->Lq * a->Hq + 3) / 4));
-  if (grid.x > (1u << 23)) { set_error("pp_shared_prefix_attention: too many queries"); return PP_ERR_ARG; }
-#define PA_LAUNCH(T, DD) hipLaunchKernelGGL((pa_simple_kernel<T, DD>), grid, dim3(256), 0, st, p)
-  if (a->dtype == PP_F16) { if (a->D == 128) PA_LAUNCH(_Float16, 128); else PA_LAUNCH(_Float16, 64); }
-  else { if (a->D == 128) PA_LAUNCH(float, 128); else PA_LAUNCH(float, 64); }
-#undef PA_LAUNCH
+  if (a->dtype == PP_F16) {
+    if (a->D == 128) pa_launch<_Float16, 128>(plan, p, st);
+    else pa_launch<_Float16, 64>(plan, p, st);
+  } else {
+    if (a->D == 128) pa_launch<float, 128>(plan, p, st);
+    else pa_launch<float, 64>(plan, p, st);
+  }
   return launch_status("pp_shared_prefix_attention");
 }
