@@ -449,7 +449,7 @@ int pp_ffn_fold_unfold(const void* in, void* out, int BT, int C, int H, int W, i
  * in / out: channel windows [choff, choff + C) of NHWC buffers of dtype (out may be `in` itself, same window); C % 8 == 0, C <= 2048,
  * groups divides C, strides and offsets multiples of 8, buffers 16-byte aligned.  act: any PP_ACT_* (slope of LRELU = act_param).
  * Channels of `out` outside its window are left as they are.  stats_ws: caller-owned fp32 workspace of
- * pp_group_norm_workspace_floats elements, 8-byte aligned.  A NaN or infinity makes its group NaN.  Deterministic. */
+ * pp_group_norm_workspace_floats elements, 8-byte aligned (0 elements: NULL will do).  A NaN or infinity makes its group NaN.  Deterministic. */
 int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, int groups);
 int pp_group_norm(const void* in, int in_cstride, int in_choff, void* out, int out_cstride, int out_choff, const float* gamma,
                   const float* beta, float* stats_ws, int N, int H, int W, int C, int groups, float eps, int act, float act_param,
@@ -473,6 +473,13 @@ int64_t pp_linear_i8_weight_bytes(int N, int K);
 int pp_linear_i8_pack(const void* wq, int64_t wq_rstride, void* weight, int N, int K, void* stream);
 int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out,
                  int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* stream);
+
+/* pp_quantize_tokens and pp_linear_i8 in one call on float tokens x (rows of K elements of x_dtype, x_rstride elements apart).  work: device
+ * scratch of pp_linear_i8_tokens_workspace_bytes(M, K) bytes, 16-byte aligned (0 for one or two tokens: one kernel does both). */
+int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int K);
+int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const void* weight, const float* ws, const float* bias, void* out,
+                        int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* work,
+                        int64_t work_bytes, void* stream);
 
 /* Attention of B sequences of Lq query tokens over the keys of a prefix shared by the B / G sequences of a group (sequence b belongs
  * to group b / (B / G)) and the keys of their own suffix: softmax(scale * q k^T) v in one softmax over both.  The windows of a frame with

@@ -415,8 +415,7 @@ class Int8Linear:
         """x [..., K] fp32 / fp16 -> [..., N] (out_dtype: default x's; a given `out` is [rows, >= N] and returned as it is)"""
         if x.shape[-1] != self.K:
             raise ValueError(f"Int8Linear: {x.shape[-1]} input channels, built for {self.K}")
-        codes, scale = hip.quantize_tokens(x)
-        y = self.product(codes, scale, act=act, act_param=act_param, out_dtype=out_dtype or x.dtype, out=out)
+        y = hip.linear_i8_tokens(x, self.weight, self.scale, self.bias, self.N, act=ACTS_I8[act], act_param=act_param, out_dtype=out_dtype, out=out)
         return y if out is not None else y.view(*x.shape[:-1], self.N)
 
 

@@ -17,7 +17,7 @@ struct GnParams {
   float* part;            // [N][slices][groups][2] (mean, M2) of a slice
   long long in_cs, out_cs;
   int in_co, out_co;
-  int HW, C, groups, cg, slices, ppslice;   // ppslice: pixels per slice
+  int HW, C, groups, cg, slices, ppslice, ppblock;   // pixels of a slice (statistics), of a block (output)
   float eps, act_param;
   int act;
 };
@@ -94,7 +94,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   __shared__ float gm[2048], gr[2048];                 // mean and rstd of every group (groups <= C <= 2048)
   __shared__ float part_n[256], part_m[256], part_v[256];
-  const int t = threadIdx.x, n = blockIdx.y;
+  // images and pixels in the opposite order of the statistics: what was read last is still in the cache
+  const int t = threadIdx.x, n = gridDim.y - 1 - blockIdx.y;
   const float* part = p.part + (long long)n * p.slices * p.groups * 2;
   const int per = p.groups < 256 ? 256 / p.groups : 1;  // threads that share one group's slices
   for (int g0 = 0; g0 < p.groups; g0 += 256) {
@@ -136,18 +137,100 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   }
   const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + col * 8;
   T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + col * 8;
-  for (long long q = (long long)blockIdx.x * rows + pr; q < p.HW; q += (long long)gridDim.x * rows) {
-    float v[8];
-    load8<T>(x + q * p.in_cs, v);
+  const long long q0 = (long long)(gridDim.x - 1 - blockIdx.x) * p.ppblock, q1 = min(q0 + p.ppblock, (long long)p.HW);
+  constexpr int U = 4;                                  // loads in flight a thread
+  for (long long q = q0 + pr; q < q1; q += U * rows) {
+    float v[U][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value(fmaf(v[i] - mean[i], mul[i], add[i]), p.act, p.act_param);
-    store8<T>(y + q * p.out_cs, v);
+    for (int u = 0; u < U; ++u)
+      if (q + u * rows < q1) load8<T>(x + (q + u * rows) * p.in_cs, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * rows < q1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = act_value(fmaf(v[u][i] - mean[i], mul[i], add[i]), p.act, p.act_param);
+        store8<T>(y + (q + u * rows) * p.out_cs, v[u]);
+      }
+  }
+}
+
+// Sum over the block, the same value in every thread; two barriers.
+template <int BLOCK>
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int w = 0; w < BLOCK / 64; ++w) v += lds[w];
+  __syncthreads();
+  return v;
+}
+
+// A group that fits a block's registers (channels of a group a multiple of 8): one launch, one read; the variance is a second pass over registers.
+constexpr int GN_VEC = 8;         // vectors of 8 a thread
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void gn_group_kernel(const GnParams p) {
+  __shared__ float red[BLOCK / 64];
+  const int g = blockIdx.x, n = blockIdx.y, vpp = p.cg >> 3, total = p.HW * vpp;
+  const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + g * p.cg;
+  T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + g * p.cg;
+  float v[GN_VEC][8];
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < GN_VEC; ++k) {
+    const int i = k * BLOCK + threadIdx.x, px = i / vpp;
+    if (i < total) {
+      load8<T>(x + px * p.in_cs + (i - px * vpp) * 8, v[k]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[k][j];
+    }
+  }
+  const float count = (float)p.HW * (float)p.cg;
+  const float mean = block_sum<BLOCK>(sum, red) / count;
+  float dev = 0.f;
+#pragma unroll
+  for (int k = 0; k < GN_VEC; ++k)
+    if (k * BLOCK + (int)threadIdx.x < total) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[k][j] -= mean;
+        dev = fmaf(v[k][j], v[k][j], dev);
+      }
+    }
+  const float rstd = 1.f / sqrtf(block_sum<BLOCK>(dev, red) / count + p.eps);
+#pragma unroll
+  for (int k = 0; k < GN_VEC; ++k) {
+    const int i = k * BLOCK + threadIdx.x, px = i / vpp;
+    if (i < total) {
+      const int c = (i - px * vpp) * 8;
+      float gm[8], bt[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { gm[j] = rstd; bt[j] = 0.f; }
+      if (p.gamma != nullptr)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gm[j] = rstd * p.gamma[g * p.cg + c + j];
+      if (p.beta != nullptr)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bt[j] = p.beta[g * p.cg + c + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = act_value(fmaf(v[k][j], gm[j], bt[j]), p.act, p.act_param);
+      store8<T>(y + px * p.out_cs + c, v[k]);
+    }
   }
 }
 
 }  // namespace pp
 
 using namespace pp;
+
+// A group in one block's registers: its share of a map is small, or there are groups enough to fill the chip.  Measured in one launch against two:
+// 30 x 54 x 128 in 8 groups FIGURE.
+static bool gn_in_registers(int64_t HW, int C, int groups) {
+  const int cg = C / groups;
+  return cg % 8 == 0 && HW * cg <= 1024 * GN_VEC * 8;
+}
 
 static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
   // enough blocks to fill the chip, but no slice under 64 vectors a column set (the joins would cost more than the pixels)
@@ -162,6 +245,7 @@ static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
 
 extern "C" int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, int groups) {
   if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 != 0 || C > 2048 || groups <= 0 || C % groups != 0 || (int64_t)H * W > 0x7fffffff) return PP_ERR_ARG;
+  if (gn_in_registers((int64_t)H * W, C, groups)) return 0;
   int slices, pps;
   gn_split(N, H * W, C, &slices, &pps);
   return (int64_t)N * slices * groups * 2;
@@ -170,7 +254,7 @@ extern "C" int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, in
 extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void* out, int out_cstride, int out_choff, const float* gamma,
                              const float* beta, float* stats_ws, int N, int H, int W, int C, int groups, float eps, int act, float act_param,
                              int dtype, void* stream) {
-  PP_REQUIRE(in && out && stats_ws && N > 0 && N <= 65535 && H > 0 && W > 0 && (int64_t)H * W <= 0x7fffffff, PP_ERR_ARG,
+  PP_REQUIRE(in && out && N > 0 && N <= 65535 && H > 0 && W > 0 && (int64_t)H * W <= 0x7fffffff, PP_ERR_ARG,
              "pp_group_norm: bad arguments (N=%d H=%d W=%d)", N, H, W);
   PP_REQUIRE(C > 0 && C % 8 == 0 && C <= 2048 && groups > 0 && C % groups == 0, PP_ERR_ARG,
              "pp_group_norm: C=%d must be a multiple of 8, <= 2048, and of groups=%d", C, groups);
@@ -183,16 +267,32 @@ extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void*
                  (uintptr_t)stats_ws % 8 == 0,
              PP_ERR_ALIGN, "pp_group_norm: strides and channel offsets must be multiples of 8, the buffers 16-byte aligned");
   const int HW = H * W;
+  const bool one = gn_in_registers(HW, C, groups);
+  PP_REQUIRE(one || stats_ws, PP_ERR_WORKSPACE, "pp_group_norm: needs %lld floats of scratch", (long long)pp_group_norm_workspace_floats(N, H, W, C, groups));
   GnParams p;
   p.in = (const char*)in; p.out = (char*)out; p.gamma = gamma; p.beta = beta; p.part = stats_ws;
   p.in_cs = in_cstride; p.out_cs = out_cstride; p.in_co = in_choff; p.out_co = out_choff;
   p.HW = HW; p.C = C; p.groups = groups; p.cg = C / groups; p.eps = eps; p.act = act; p.act_param = act_param;
-  gn_split(N, HW, C, &p.slices, &p.ppslice);
   hipStream_t st = (hipStream_t)stream;
+  if (one) {
+    const dim3 grid(groups, N);
+    const bool small = (int64_t)HW * p.cg <= 256 * GN_VEC * 8;
+    if (dtype == PP_F16) {
+      if (small) hipLaunchKernelGGL((gn_group_kernel<_Float16, 256>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((gn_group_kernel<_Float16, 1024>), grid, dim3(1024), 0, st, p);
+    } else {
+      if (small) hipLaunchKernelGGL((gn_group_kernel<float, 256>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((gn_group_kernel<float, 1024>), grid, dim3(1024), 0, st, p);
+    }
+    return launch_status("pp_group_norm");
+  }
+  gn_split(N, HW, C, &p.slices, &p.ppslice);
   const int rows = 256 / (C / 8);
-  int blocks = ceil_div(HW, rows);
+  int blocks = ceil_div(HW, 4 * rows);
   const int most = 2048 / N > 1 ? 2048 / N : 1;
   if (blocks > most) blocks = most;
+  p.ppblock = ceil_div(HW, blocks);
+  blocks = ceil_div(HW, p.ppblock);
   if (dtype == PP_F16) {
     hipLaunchKernelGGL((gn_stats_kernel<_Float16>), dim3(p.slices, N), dim3(256), 0, st, p);
     hipLaunchKernelGGL((gn_apply_kernel<_Float16>), dim3(blocks, N), dim3(256), 0, st, p);

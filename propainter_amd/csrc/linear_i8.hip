@@ -71,9 +71,19 @@ __device__ __forceinline__ u32x2 codes8(const float* v, const RowScale& r) {
   return u32x2{w[0], w[1]};
 }
 
+// maximum over the wave, on the VALU: rotations inside the 16-lane rows, then the swaps of rows and half-waves
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+#if defined(__HIP_DEVICE_COMPILE__)
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));      // row_ror:8, 4, 2, 1
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  u2 r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max((unsigned)r.x, (unsigned)r.y);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max((unsigned)r.x, (unsigned)r.y);
+#endif
   return v;
 }
 
@@ -137,51 +147,70 @@ template <> struct Raw8<float> {
   }
 };
 
-// A row in the registers of WPR waves, VPL vectors of 8 a lane: one pass over memory.  4 / WPR rows a block.
-template <typename T, int VPL, int WPR>
+__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
+
+// R rows in the registers of WPR waves, VPL vectors of 8 a lane and row: one pass over memory.  4 R / WPR rows a block.
+template <typename T, int VPL, int WPR, int R>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, long long xrs, int8_t* __restrict__ q, long long qrs,
                                                     float* __restrict__ scale, long long rows, int K, int Kp, int wide) {
   __shared__ unsigned wm[4];
   const int wave = threadIdx.x >> 6, t = threadIdx.x % (64 * WPR);
-  for (long long row0 = blockIdx.x * (long long)(4 / WPR); row0 < rows; row0 += gridDim.x * (long long)(4 / WPR)) {
-    const long long row = row0 + wave / WPR;
-    const bool on = row < rows;
-    const T* xr = x + (on ? row : rows - 1) * xrs;
-    Raw8<T> raw[VPL];
-    unsigned m = 0;
+  constexpr int RB = 4 * R / WPR;
+  for (long long row0 = blockIdx.x * (long long)RB; row0 < rows; row0 += gridDim.x * (long long)RB) {
+    Raw8<T> raw[R][VPL];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      const int c = (v * 64 * WPR + t) * 8;
-      if (wide && c + 8 <= K) {
-        raw[v].load(xr + c);
-      } else {
+    for (int k = 0; k < R; ++k) {
+      const long long row = min(row0 + wave / WPR * R + k, rows - 1);
+      const T* xr = x + row * xrs;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < K ? xr[c + i] : (T)0.f);
+      for (int v = 0; v < VPL; ++v) {
+        const int c = (v * 64 * WPR + t) * 8;
+        if (wide && c + 8 <= K) {
+          raw[k][v].load(xr + c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) raw[k][v].set(i, c + i < K ? xr[c + i] : (T)0.f);
+        }
       }
     }
+    unsigned mine = 0;                             // lane k: the maximum of row k, so that one division sequence serves R rows
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) m = max(m, raw[v].amax());
-    m = wave_umax(m);
+    for (int k = 0; k < R; ++k) {
+      unsigned m = 0;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) m = max(m, raw[k][v].amax());
+      m = wave_umax(m);
+      if (R == 1 || (threadIdx.x & 63) == k) mine = m;
+    }
     if constexpr (WPR == 4) {
-      if ((threadIdx.x & 63) == 0) wm[wave] = m;
+      if ((threadIdx.x & 63) == 0) wm[wave] = mine;
       __syncthreads();
-      m = max(max(wm[0], wm[1]), max(wm[2], wm[3]));
+      mine = max(max(wm[0], wm[1]), max(wm[2], wm[3]));
       __syncthreads();
     }
-    m = __builtin_amdgcn_readfirstlane(m);
-    const RowScale r = row_scale(m);
-    if (!on) continue;                                     // (WPR == 4: one row a block, always on)
-    if (t == 0) scale[row] = r.scale;
-    const bool plain = !r.zero && r.lift == 1.f;
-    const float half = 0.5f * r.s;
-    int8_t* qr = q + row * qrs;
+    const RowScale all = row_scale(mine);
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      const int c = (v * 64 * WPR + t) * 8;
-      if (c >= Kp) break;
-      float f[8];
-      raw[v].values(f);
-      *reinterpret_cast<u32x2*>(qr + c) = plain ? codes8_fast(f, r, half) : codes8(f, r);
+    for (int k = 0; k < R; ++k) {
+      const long long row = row0 + wave / WPR * R + k;
+      if (row >= rows) break;                              // (WPR == 4: one row a block, always below)
+      RowScale r;
+      r.scale = lane_of(all.scale, k);
+      r.s = lane_of(all.s, k);
+      r.rcp = lane_of(all.rcp, k);
+      r.lift = lane_of(all.lift, k);
+      r.zero = __builtin_amdgcn_readlane((int)all.zero, k) != 0;
+      if (t == 0) scale[row] = r.scale;
+      const bool plain = !r.zero && r.lift == 1.f;
+      const float half = 0.5f * r.s;
+      int8_t* qr = q + row * qrs;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const int c = (v * 64 * WPR + t) * 8;
+        if (c >= Kp) break;
+        float f[8];
+        raw[k][v].values(f);
+        *reinterpret_cast<u32x2*>(qr + c) = plain ? codes8_fast(f, r, half) : codes8(f, r);
+      }
     }
   }
 }
@@ -253,83 +282,188 @@ struct LinI8Params {
   int wide_out;      // rows of `out` are 16-byte aligned
 };
 
-// The channels of a 64-channel block that one lane holds (8 at c0 = n0 + (lane / 16) * 8, 8 at c0 + 32) with their scales and biases
-template <typename TO> struct LaneChannels {
-  int c0;
-  float ws[16], bias[16];
-  __device__ __forceinline__ void load(const LinI8Params& p, int n0) {
-    c0 = n0 + ((threadIdx.x & 63) >> 4) * 8;
+// 8 consecutive channels c .. c + 7 that a lane holds of two neighbouring operand tiles, with their scales and biases
+template <typename TO> struct Lane8 {
+  int c;
+  float ws[8], bias[8];
+  __device__ __forceinline__ void load(const LinI8Params& p, int first) {
+    c = first;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int n = min(c0 + (i >> 3) * 32 + (i & 7), p.N - 1);
+    for (int i = 0; i < 8; ++i) {
+      const int n = min(c + i, p.N - 1);
       ws[i] = p.ws[n];
       bias[i] = p.bias != nullptr ? p.bias[n] : 0.f;
     }
   }
-  // scale, bias, activation, store of token m
-  __device__ __forceinline__ void store(const LinI8Params& p, long long m, float xs, const i32x4* acc) const {
-    TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c0;
+  // scale, bias, activation
+  __device__ __forceinline__ void value(const LinI8Params& p, float xs, const i32x4* acc, float* v) const {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[8];
+    for (int i = 0; i < 8; ++i) v[i] = fmaf((float)acc[i >> 2][i & 3] * xs, ws[i], bias[i]);
+    if (p.act != PP_ACT_NONE) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf((float)acc[h * 2 + (i >> 2)][i & 3] * xs, ws[h * 8 + i], bias[h * 8 + i]);
-      if (p.act != PP_ACT_NONE) {
+      for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], p.act, p.act_param);
+    }
+  }
+  __device__ __forceinline__ void store(const LinI8Params& p, long long m, const float* v) const {
+    TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c;
+    if (p.wide_out && c + 8 <= p.N) {
+      store8<TO>(o, v);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], p.act, p.act_param);
-      }
-      const int c = c0 + h * 32;
-      if (p.wide_out && c + 8 <= p.N) {
-        store8<TO>(o + h * 32, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < p.N) o[h * 32 + i] = from_f32<TO>(v[i]);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (c + i < p.N) o[i] = from_f32<TO>(v[i]);
     }
   }
 };
 
-// 4 waves, each 64 channels x 32 tokens, operands straight from memory.  Token rows past M repeat the last one and are not stored.
-template <typename TO>
-__global__ __launch_bounds__(256) void lin_i8_kernel(const LinI8Params p) {
+// Few tokens: the weights' bytes are the work.  A block takes TPB operand tiles (16 channels each) of one 64-channel block and 16 MT tokens; its 8
+// waves share out K, operands straight from memory, several tiles in flight, and add their exact partial sums through LDS.
+constexpr int I8_KW = 8;
+template <typename T> struct FloatTokens { const T* x; long long xrs; int K, wide; };
+
+// acc[t][j] += tiles kt0 .. kt1 of the weights times the tokens; tok(kt, j) gives the token operand
+template <int MT, int TPB, typename F>
+__device__ __forceinline__ void thin_product(const u32x4* w, int kt0, int kt1, i32x4 (&acc)[TPB][MT], F tok) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long m0 = (blockIdx.x * 4ll + wave) * 32;
-  const int nb = blockIdx.y;
-  const u32x4* w = p.w + (long long)nb * p.ktiles * 256 + lane;
-  const int8_t* xa[2];
+  constexpr int U = TPB + MT <= 3 ? 8 : 4;
+  int kt = kt0;
+  for (; kt + U <= kt1; kt += U) {
+    i32x4 wf[U][TPB], xf[U][MT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    long long m = m0 + j * 16 + (lane & 15);
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int t = 0; t < TPB; ++t) wf[u][t] = __builtin_bit_cast(i32x4, w[(long long)(kt + u) * 256 + t * 64]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) xf[u][j] = tok(kt + u, j);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < TPB; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][t], xf[u][j], acc[t][j], 0, 0, 0);
+  }
+  for (; kt < kt1; ++kt)
+#pragma unroll
+    for (int t = 0; t < TPB; ++t) {
+      const i32x4 wf = __builtin_bit_cast(i32x4, w[(long long)kt * 256 + t * 64]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, tok(kt, j), acc[t][j], 0, 0, 0);
+    }
+#endif
+}
+
+// adds the waves' sums and writes the block's outputs; xs_of(m) is the scale of token m
+template <typename TO, int MT, int TPB, typename F>
+__device__ __forceinline__ void thin_finish(const LinI8Params& p, i32x4* red, const i32x4 (&acc)[TPB][MT], int nb, int t0, long long m0, F xs_of) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int t = 0; t < TPB; ++t)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[((t * MT + j) * I8_KW + wave) * 64 + lane] = acc[t][j];
+  __syncthreads();
+  for (int f = wave; f < TPB * MT; f += I8_KW) {
+    i32x4 a = red[f * I8_KW * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < I8_KW; ++w) a += red[(f * I8_KW + w) * 64 + lane];
+    const int t = t0 + f / MT;
+    const long long m = m0 + f % MT * 16 + (lane & 15);
+    const int c = nb * 64 + (t >> 1) * 32 + (lane >> 4) * 8 + (t & 1) * 4;
+    if (m >= p.M) continue;
+    const float xs = xs_of(m);
+    TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < p.N)
+        o[i] = from_f32<TO>(act_value(fmaf((float)a[i] * xs, p.ws[c + i], p.bias != nullptr ? p.bias[c + i] : 0.f), p.act, p.act_param));
+  }
+}
+
+template <typename TO, int MT, int TPB>
+__global__ __launch_bounds__(512) void lin_i8_thin_kernel(const LinI8Params p) {
+  __shared__ __attribute__((aligned(16))) i32x4 red[TPB * MT * I8_KW * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nb = blockIdx.x / (4 / TPB), t0 = blockIdx.x % (4 / TPB) * TPB;
+  const long long m0 = blockIdx.y * 16ll * MT;
+  const u32x4* w = p.w + (long long)nb * p.ktiles * 256 + t0 * 64 + lane;
+  const int8_t* xa[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    long long m = m0 + j * 16 + (lane & 15);      // token rows past M repeat the last one and are not stored
     if (m >= p.M) m = p.M - 1;
     xa[j] = p.xq + m * p.qrs + (lane >> 4) * 16;
   }
-  i32x4 acc[2][4];
+  i32x4 acc[TPB][MT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int t = 0; t < TPB; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[j][t] = i32x4{0, 0, 0, 0};
-  for (int kt = 0; kt < p.ktiles; ++kt) {
-    u32x4 wf[4];
+    for (int j = 0; j < MT; ++j) acc[t][j] = i32x4{0, 0, 0, 0};
+  thin_product<MT, TPB>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
+                        [&](int kt, int j) { return *reinterpret_cast<const i32x4*>(xa[j] + (long long)kt * 64); });
+  thin_finish<TO, MT, TPB>(p, red, acc, nb, t0, m0, [&](long long m) { return p.xs[m]; });
+}
+
+// One or two float tokens (M * ceil(K / 4096) <= 2): every block makes their codes itself, into LDS -- they come out of L2, and a launch and a
+// round trip of the codes are saved.  4096 -> 4096: one token 8.0 us against 7.0 for the product alone plus a launch for the codes; four tokens
+// 10.4, no gain any more.
+constexpr int I8_FUSE = 2;
+inline bool i8_fused(int64_t M, int K) { return M * ((K + 4095) / 4096) <= I8_FUSE; }
+template <typename T, typename TO>
+__global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, const FloatTokens<T> x) {
+  constexpr int TPB = 1;
+  __shared__ __attribute__((aligned(16))) i32x4 red[TPB * I8_KW * 64];
+  __shared__ __attribute__((aligned(16))) int8_t codes[I8_FUSE * (4096 + 16)];
+  __shared__ unsigned wmax[I8_FUSE][8];
+  __shared__ float xs[I8_FUSE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nb = blockIdx.x / (4 / TPB), t0 = blockIdx.x % (4 / TPB) * TPB;
+  const int M = (int)p.M, Kp = p.ktiles * 64, per = (x.K + 4095) / 4096, ld = per * 4096 + 16;      // M * ld <= sizeof(codes)
+  Raw8<T> raw[I8_FUSE];                            // vector v = token v / per, columns (v % per) * 4096 + thread * 8 ..
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wf[t] = w[(long long)kt * 256 + t * 64];
+  for (int v = 0; v < I8_FUSE; ++v) {
+    if (v >= M * per) break;
+    const T* xr = x.x + (long long)(v / per) * x.xrs;
+    const int c = v % per * 4096 + threadIdx.x * 8;
+    if (x.wide && c + 8 <= x.K) {
+      raw[v].load(xr + c);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const u32x4 xf = *reinterpret_cast<const u32x4*>(xa[j] + (long long)kt * 64);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        acc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[t]), __builtin_bit_cast(i32x4, xf), acc[j][t], 0, 0, 0);
+      for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < x.K ? xr[c + i] : (T)0.f);
     }
   }
-  LaneChannels<TO> ch;
-  ch.load(p, nb * 64);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const long long m = m0 + j * 16 + (lane & 15);
-    if (m < p.M) ch.store(p, m, p.xs[m], acc[j]);
+  for (int v = 0; v < I8_FUSE; ++v) {
+    if (v >= M * per) break;
+    const unsigned m = wave_umax(raw[v].amax());
+    if (lane == 0) wmax[v][wave] = m;
   }
-#endif
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < I8_FUSE; ++v) {
+    if (v >= M * per) break;
+    const int row = v / per;
+    unsigned m = 0;
+    for (int k = row * per; k < (row + 1) * per; ++k)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = max(m, wmax[k][w]);
+    m = __builtin_amdgcn_readfirstlane(m);
+    const RowScale r = row_scale(m);
+    if (threadIdx.x == 0) xs[row] = r.scale;
+    const int c = v % per * 4096 + threadIdx.x * 8;
+    float f[8];
+    raw[v].values(f);
+    if (c < Kp) *reinterpret_cast<u32x2*>(codes + row * ld + c) = !r.zero && r.lift == 1.f ? codes8_fast(f, r, 0.5f * r.s) : codes8(f, r);
+  }
+  __syncthreads();
+  i32x4 acc[TPB][1];
+#pragma unroll
+  for (int t = 0; t < TPB; ++t) acc[t][0] = i32x4{0, 0, 0, 0};
+  const u32x4* w = p.w + (long long)nb * p.ktiles * 256 + t0 * 64 + lane;
+  const bool on = (lane & 15) < M;
+  const int8_t* xa = codes + (on ? lane & 15 : 0) * ld + (lane >> 4) * 16;
+  thin_product<1, TPB>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
+                       [&](int kt, int) { return *reinterpret_cast<const i32x4*>(xa + kt * 64); });
+  thin_finish<TO, 1, TPB>(p, red, acc, nb, t0, 0, [&](long long m) { return xs[m]; });
 }
 
 // Tiles of BM tokens x BN channels, WM x WN waves of BM / WM tokens x BN / WN channels.  Both operands go from memory into LDS without
@@ -339,8 +473,8 @@ __global__ __launch_bounds__(256) void lin_i8_kernel(const LinI8Params p) {
 typedef __attribute__((address_space(3))) void* i8_lptr;
 typedef __attribute__((address_space(1))) void* i8_gptr;
 
-template <typename TO, int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN, 1) void lin_i8_tile_kernel(const LinI8Params p, const int tm, const int tn) {
+template <typename TO, int BM, int BN, int WM, int WN, int S, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void lin_i8_tile_kernel(const LinI8Params p, const int tm, const int tn) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = WM * WN, PA = BM / 16, PW = BN / 16, G = (PA + PW) / NW;      // 1 KB pieces of a stage; DMA instructions a wave
   constexpr int STAGE = (PA + PW) * 1024, TA = BM / WM / 16, TB = BN / WN / 64;    // 16-token tiles, 64-channel blocks of a wave
@@ -416,32 +550,134 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void lin_i8_tile_kernel(const LinI
     buf = buf + 1 == S ? 0 : buf + 1;
     nbuf = nbuf + 1 == S ? 0 : nbuf + 1;
   }
+  float xs[TA];      // all scales ahead of the first store: a load between stores would wait for them (one in-order counter)
+#pragma unroll
+  for (int a = 0; a < TA; ++a) xs[a] = p.xs[min(m0 + (wm * TA + a) * 16 + (lane & 15), p.M - 1)];
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
-    const int nb = n0 + (wn * TB + b) * 64;
-    if (nb >= p.N) break;
-    LaneChannels<TO> ch;
-    ch.load(p, nb);
+    Lane8<TO> ch[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) ch[h].load(p, n0 + (wn * TB + b) * 64 + h * 32 + (lane >> 4) * 8);
 #pragma unroll
     for (int a = 0; a < TA; ++a) {
       const long long m = m0 + (wm * TA + a) * 16 + (lane & 15);
-      if (m < p.M) ch.store(p, m, p.xs[m], &acc[a][b * 4]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        ch[h].value(p, xs[a], &acc[a][b * 4 + h * 2], v);
+        if (m < p.M) ch[h].store(p, m, v);
+      }
     }
   }
 #endif
 }
 
-template <typename TO, int BM, int BN, int WM, int WN, int S>
+// Short K, many tokens: the output's bytes are the work.  A block of 4 waves keeps the weights of 256 channels in registers (64 a wave, KT operand
+// tiles deep) for the whole launch and streams token tiles of 64 through two LDS stages.  The `panels` blocks that read the same tokens
+// run next to each other on one XCD (block id mod 8).
+template <typename TO, int KT>
+__global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params p, const int panels, const int groups, const int tiles) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ __attribute__((aligned(1024))) char lds[2 * 4 * KT * 1024];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int panel = (int)(blockIdx.x >> 3) % panels, grp = (int)(blockIdx.x >> 3) / panels * 8 + (int)(blockIdx.x & 7);
+  const int nb = panel * 4 + wave, last = (p.N + 63) / 64 - 1;
+  i32x4 wf[KT][4];
+  {
+    const u32x4* w = p.w + (long long)(nb < last ? nb : last) * p.ktiles * 256 + lane;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) wf[kt][t] = kt < p.ktiles ? __builtin_bit_cast(i32x4, w[kt * 256 + t * 64]) : i32x4{0, 0, 0, 0};
+  }
+  Lane8<TO> ch[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) ch[h].load(p, nb * 64 + h * 32 + (lane >> 4) * 8);
+  float xs[4], xn[4];                              // scales of this tile's and the next tile's tokens: a load between the stores would wait for them
+  auto issue = [&](int tile, int buf) {
+    long long m = tile * 64ll + wave * 16 + (lane & 15);
+    if (m >= p.M) m = p.M - 1;
+    const int8_t* src = p.xq + m * p.qrs + (lane >> 4) * 16;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+      if (kt < p.ktiles) __builtin_amdgcn_global_load_lds((i8_gptr)(src + kt * 64), (i8_lptr)(lds + ((buf * 4 + wave) * KT + kt) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) xn[mt] = p.xs[min(tile * 64ll + mt * 16 + (lane & 15), p.M - 1)];
+  };
+  int buf = 0;
+  if (grp < tiles) issue(grp, 0);
+  for (int tile = grp; tile < tiles; tile += groups) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                  // tile is there for all waves; the other stage, read one tile ago, is free
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) xs[mt] = xn[mt];
+    if (tile + groups < tiles) issue(tile + groups, buf ^ 1);
+    const char* st = lds + buf * 4 * KT * 1024 + lane * 16;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      i32x4 acc[4], xf[KT];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[t] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) xf[kt] = kt < p.ktiles ? *reinterpret_cast<const i32x4*>(st + (mt * KT + kt) * 1024) : i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[kt][t], xf[kt], acc[t], 0, 0, 0);
+      const long long m = tile * 64ll + mt * 16 + (lane & 15);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        ch[h].value(p, xs[mt], &acc[h * 2], v);
+        if (m < p.M) ch[h].store(p, m, v);
+      }
+    }
+    buf ^= 1;
+  }
+#endif
+}
+template <typename TO, int KT>
+static void launch_stream(const LinI8Params& p, hipStream_t st) {
+  const int panels = (p.N + 255) / 256, tiles = (int)((p.M + 63) / 64);
+  int per = 64 / panels;                           // token groups an XCD works on at a time: 64 blocks, two a CU
+  if (per < 1) per = 1;
+  hipLaunchKernelGGL((lin_i8_stream_kernel<TO, KT>), dim3((unsigned)(8 * panels * per)), dim3(256), 0, st, p, panels, 8 * per, tiles);
+}
+
+template <typename TO, int BM, int BN, int WM, int WN, int S, int OCC>
 static void launch_tiles(const LinI8Params& p, hipStream_t st) {
   const int tm = (int)((p.M + BM - 1) / BM), tn = (p.N + BN - 1) / BN;
-  hipLaunchKernelGGL((lin_i8_tile_kernel<TO, BM, BN, WM, WN, S>), dim3((unsigned)((long long)tm * tn)), dim3(64 * WM * WN), 0, st, p, tm, tn);
+  hipLaunchKernelGGL((lin_i8_tile_kernel<TO, BM, BN, WM, WN, S, OCC>), dim3((unsigned)((long long)tm * tn)), dim3(64 * WM * WN), 0, st, p, tm, tn);
 }
+template <typename TO, int MT, int TPB>
+static void launch_thin(const LinI8Params& p, hipStream_t st) {
+  hipLaunchKernelGGL((lin_i8_thin_kernel<TO, MT, TPB>), dim3((unsigned)((p.N + 63) / 64 * (4 / TPB)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, p);
+}
+// Which form: measured at K = N = 4096 unless said otherwise (us).
+//   thin, few 128 x 128 tiles (at most 64: they would leave most CUs idle) or few tokens: 16 tokens x 1024 -> 16384 6.0 against 8.5 with tiles, 64 tokens 10.5 against 22.7 with tiles, 256 tokens 15.5 against 23.3,
+//   512 tokens 28.7 against 23.8
+//   stream, K <= 512 and enough token tiles for every resident block: 110160 x 512 -> 1536 134 against 166, 10000 tokens 16.4 against 17.3,
+//   5000 x 512 -> 512 7.9 against 6.8
+//   256 x 256 tiles where K is long and they fill the chip twice: 8192^3 487 against 505 with 128 x 256; 4096^3 65 either way
+//   128 x 256 tiles where they fill the chip: 4096^3 66 against 84 with 128 x 128; 2048^3 20.5 against 15.4
 template <typename TO>
 static void launch_product(const LinI8Params& p, hipStream_t st) {
-  const long long t256 = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (p.M <= 32) hipLaunchKernelGGL((lin_i8_kernel<TO>), dim3((unsigned)((p.M + 127) / 128), (p.N + 63) / 64), dim3(256), 0, st, p);
-  else if (t256 >= 256) launch_tiles<TO, 256, 256, 2, 4, 4>(p, st);
-  else launch_tiles<TO, 128, 128, 2, 2, 4>(p, st);
+  const long long t128 = ((p.M + 127) / 128) * ((p.N + 127) / 128), t256w = ((p.M + 127) / 128) * ((p.N + 255) / 256), t256 = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (t128 <= 64 || p.M <= 32) {
+    if (p.M <= 16) launch_thin<TO, 1, 1>(p, st);
+    else if (p.M <= 32) launch_thin<TO, 1, 2>(p, st);
+    else if (p.M <= 64) launch_thin<TO, 1, 4>(p, st);
+    else launch_thin<TO, 2, 4>(p, st);
+  } else if (p.ktiles <= 8 && (p.M + 63) / 64 * ((p.N + 255) / 256) >= 768) {
+    if (p.ktiles <= 4) launch_stream<TO, 4>(p, st);
+    else launch_stream<TO, 8>(p, st);
+  } else if (p.ktiles >= 96 && t256 >= 512) {
+    launch_tiles<TO, 256, 256, 2, 4, 4, 1>(p, st);
+  } else if (t256w >= 256) {
+    launch_tiles<TO, 128, 256, 2, 4, 3, 1>(p, st);
+  } else {
+    launch_tiles<TO, 128, 128, 4, 2, 4, 1>(p, st);
+  }
 }
 
 }  // namespace pp
@@ -460,14 +696,19 @@ extern "C" int pp_i8_row_bytes(int K) {
 template <typename T>
 static void launch_quant(const void* x, int64_t xrs, void* q, int64_t qrs, float* scale, int64_t rows, int K, int Kp, int wide, hipStream_t st) {
   const int64_t want = K <= 2048 ? (rows + 3) / 4 : rows;
-  const dim3 grid((unsigned)(want < 65536 ? want : 65536)), block(256);
-#define PP_QUANT(V, W) hipLaunchKernelGGL((quant_kernel<T, V, W>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide)
-  if (K <= 512) PP_QUANT(1, 1);
-  else if (K <= 1024) PP_QUANT(2, 1);
-  else if (K <= 2048) PP_QUANT(4, 1);
-  else if (K <= 4096) PP_QUANT(2, 4);
-  else if (K <= 8192) PP_QUANT(4, 4);
-  else if (K <= 16384) PP_QUANT(8, 4);
+  dim3 grid((unsigned)(want < 65536 ? want : 65536)), block(256);
+#define PP_QUANT(V, W, R) hipLaunchKernelGGL((quant_kernel<T, V, W, R>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide)
+  if (K <= 1024 && rows >= 32768) {                // enough rows to fill the chip with several in flight a wave
+    grid.x = (unsigned)((want + 3) / 4 < 65536 ? (want + 3) / 4 : 65536);
+    if (K <= 512) PP_QUANT(1, 1, 4);
+    else PP_QUANT(2, 1, 4);
+  }
+  else if (K <= 512) PP_QUANT(1, 1, 1);
+  else if (K <= 1024) PP_QUANT(2, 1, 1);
+  else if (K <= 2048) PP_QUANT(4, 1, 1);
+  else if (K <= 4096) PP_QUANT(2, 4, 1);
+  else if (K <= 8192) PP_QUANT(4, 4, 1);
+  else if (K <= 16384) PP_QUANT(8, 4, 1);
   else hipLaunchKernelGGL((quant_row_kernel<T>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide);
 #undef PP_QUANT
 }
@@ -506,25 +747,69 @@ extern "C" int pp_linear_i8_pack(const void* wq, int64_t wq_rstride, void* weigh
   return launch_status("pp_linear_i8_pack");
 }
 
-extern "C" int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out,
-                            int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* stream) {
-  const int Kp = pp_i8_row_bytes(K);
-  PP_REQUIRE(Kp > 0 && N > 0 && N <= PP_I8_MAX_N && M >= 0 && M <= PP_I8_MAX_M, PP_ERR_ARG, "pp_linear_i8: bad arguments (M=%lld N=%d K=%d)", (long long)M, N, K);
-  PP_REQUIRE(act >= PP_ACT_NONE && act <= PP_ACT_SILU, PP_ERR_ARG, "pp_linear_i8: activation code %d", act);
-  PP_REQUIRE(out_dtype == PP_F32 || out_dtype == PP_F16, PP_ERR_DTYPE, "pp_linear_i8: out_dtype %d", out_dtype);
+static int lin_i8_check(const char* who, const void* weight, const float* ws, const void* out, int64_t out_rstride, int64_t M, int N, int K, int act, int out_dtype) {
+  PP_REQUIRE(pp_i8_row_bytes(K) > 0 && N > 0 && N <= PP_I8_MAX_N && M >= 0 && M <= PP_I8_MAX_M, PP_ERR_ARG, "%s: bad arguments (M=%lld N=%d K=%d)", who, (long long)M, N, K);
+  PP_REQUIRE(act >= PP_ACT_NONE && act <= PP_ACT_SILU, PP_ERR_ARG, "%s: activation code %d", who, act);
+  PP_REQUIRE(out_dtype == PP_F32 || out_dtype == PP_F16, PP_ERR_DTYPE, "%s: out_dtype %d", who, out_dtype);
   if (M == 0) return 0;
-  PP_REQUIRE(xq && xs && weight && ws && out && q_rstride >= Kp && out_rstride >= N, PP_ERR_ARG,
-             "pp_linear_i8: null buffer or row stride (q %lld < %d, out %lld < %d)", (long long)q_rstride, Kp, (long long)out_rstride, N);
-  const int osz = out_dtype == PP_F16 ? 2 : 4;
-  PP_REQUIRE((uintptr_t)xq % 16 == 0 && q_rstride % 16 == 0 && (uintptr_t)weight % 16 == 0 && (uintptr_t)out % osz == 0, PP_ERR_ALIGN,
-             "pp_linear_i8: codes, their row stride and the weight must be multiples of 16 bytes");
+  PP_REQUIRE(weight && ws && out && out_rstride >= N, PP_ERR_ARG, "%s: null buffer or row stride (out %lld < %d)", who, (long long)out_rstride, N);
+  PP_REQUIRE((uintptr_t)weight % 16 == 0 && (uintptr_t)out % (out_dtype == PP_F16 ? 2 : 4) == 0, PP_ERR_ALIGN, "%s: the weight must be 16-byte aligned", who);
+  PP_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= (1 << 23), PP_ERR_ARG, "%s: too many tiles (M=%lld N=%d)", who, (long long)M, N);
+  return 0;
+}
+static LinI8Params lin_i8_params(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out, int64_t out_rstride,
+                                 int64_t M, int N, int K, int act, float act_param, int out_dtype) {
   LinI8Params p;
   p.xq = (const int8_t*)xq; p.xs = xs; p.w = (const u32x4*)weight; p.ws = ws; p.bias = bias; p.out = (char*)out;
-  p.qrs = q_rstride; p.ors = out_rstride; p.M = M; p.N = N; p.ktiles = Kp / 64; p.act = act; p.act_param = act_param;
-  p.wide_out = (uintptr_t)out % 16 == 0 && out_rstride * osz % 16 == 0;
-  hipStream_t st = (hipStream_t)stream;
-  PP_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= (1 << 23), PP_ERR_ARG, "pp_linear_i8: too many tiles (M=%lld N=%d)", (long long)M, N);
-  if (out_dtype == PP_F16) launch_product<_Float16>(p, st);
-  else launch_product<float>(p, st);
+  p.qrs = q_rstride; p.ors = out_rstride; p.M = M; p.N = N; p.ktiles = pp_i8_row_bytes(K) / 64; p.act = act; p.act_param = act_param;
+  p.wide_out = (uintptr_t)out % 16 == 0 && out_rstride * (out_dtype == PP_F16 ? 2 : 4) % 16 == 0;
+  return p;
+}
+
+extern "C" int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out,
+                            int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* stream) {
+  const int rc = lin_i8_check("pp_linear_i8", weight, ws, out, out_rstride, M, N, K, act, out_dtype);
+  if (rc != 0 || M == 0) return rc;
+  const int Kp = pp_i8_row_bytes(K);
+  PP_REQUIRE(xq && xs && q_rstride >= Kp, PP_ERR_ARG, "pp_linear_i8: null codes or row stride (%lld < %d)", (long long)q_rstride, Kp);
+  PP_REQUIRE((uintptr_t)xq % 16 == 0 && q_rstride % 16 == 0, PP_ERR_ALIGN, "pp_linear_i8: codes and their row stride must be multiples of 16 bytes");
+  const LinI8Params p = lin_i8_params(xq, q_rstride, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype);
+  if (out_dtype == PP_F16) launch_product<_Float16>(p, (hipStream_t)stream);
+  else launch_product<float>(p, (hipStream_t)stream);
   return launch_status("pp_linear_i8");
+}
+
+extern "C" int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int K) {
+  const int Kp = pp_i8_row_bytes(K);
+  if (Kp <= 0 || M < 0 || M > PP_I8_MAX_M) return PP_ERR_ARG;
+  return i8_fused(M, K) ? 0 : M * Kp + M * 4;
+}
+
+extern "C" int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const void* weight, const float* ws, const float* bias, void* out,
+                                   int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* work,
+                                   int64_t work_bytes, void* stream) {
+  int rc = lin_i8_check("pp_linear_i8_tokens", weight, ws, out, out_rstride, M, N, K, act, out_dtype);
+  if (rc != 0) return rc;
+  PP_REQUIRE(x_dtype == PP_F32 || x_dtype == PP_F16, PP_ERR_DTYPE, "pp_linear_i8_tokens: dtype %d", x_dtype);
+  if (M == 0) return 0;
+  const int esz = x_dtype == PP_F16 ? 2 : 4, Kp = pp_i8_row_bytes(K);
+  PP_REQUIRE(x && x_rstride >= 0, PP_ERR_ARG, "pp_linear_i8_tokens: null tokens or row stride %lld", (long long)x_rstride);
+  PP_REQUIRE((uintptr_t)x % esz == 0, PP_ERR_ALIGN, "pp_linear_i8_tokens: misaligned tokens");
+  const int64_t need = pp_linear_i8_tokens_workspace_bytes(M, K);
+  PP_REQUIRE(need == 0 || (work != nullptr && work_bytes >= need && (uintptr_t)work % 16 == 0), PP_ERR_WORKSPACE,
+             "pp_linear_i8_tokens: needs %lld bytes of 16-byte aligned scratch, got %lld", (long long)need, (long long)work_bytes);
+  int8_t* q = (int8_t*)work;
+  float* xs = (float*)(q + M * Kp);
+  if (need != 0) {
+    if ((rc = pp_quantize_tokens(x, x_rstride, q, Kp, xs, M, K, x_dtype, stream)) != 0) return rc;
+    return pp_linear_i8(q, Kp, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype, stream);
+  }
+  const LinI8Params p = lin_i8_params(nullptr, 0, nullptr, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype);
+  const int wide = (uintptr_t)x % 16 == 0 && x_rstride * esz % 16 == 0;
+  const dim3 grid((unsigned)((N + 63) / 64 * 4)), block(512);
+#define PP_TOKEN(T, TO) hipLaunchKernelGGL((lin_i8_token_kernel<T, TO>), grid, block, 0, (hipStream_t)stream, p, FloatTokens<T>{(const T*)x, (long long)x_rstride, K, wide})
+  if (x_dtype == PP_F16) { if (out_dtype == PP_F16) PP_TOKEN(_Float16, _Float16); else PP_TOKEN(_Float16, float); }
+  else { if (out_dtype == PP_F16) PP_TOKEN(float, _Float16); else PP_TOKEN(float, float); }
+#undef PP_TOKEN
+  return launch_status("pp_linear_i8_tokens");
 }

@@ -5,7 +5,9 @@ loaded or if a tensor is not on a GPU.  Tensors are passed as raw ``data_ptr()``
 all work is enqueued on torch's current stream of the device that owns the tensors.
 """
 import ctypes as C
+import functools
 import os
+import struct
 
 import numpy as np
 import torch
@@ -72,6 +74,16 @@ class PrefixAttnArgs(C.Structure):
     ]
 
 
+# argument types of the token operators' entry points: p pointer, i int32, l int64, f float
+_CTYPES = {"p": C.c_void_p, "i": C.c_int, "l": C.c_int64, "f": C.c_float}
+_TOKEN_OPS = {
+    "pp_group_norm_workspace_floats": ("l", "iiiii"), "pp_group_norm": ("i", "piipiipppiiiiififip"),
+    "pp_i8_row_bytes": ("i", "i"), "pp_quantize_tokens": ("i", "plplpliip"), "pp_linear_i8_weight_bytes": ("l", "ii"),
+    "pp_linear_i8_pack": ("i", "plpiip"), "pp_linear_i8": ("i", "plppppplliiifip"), "pp_linear_i8_tokens_workspace_bytes": ("l", "li"),
+    "pp_linear_i8_tokens": ("i", "plippppl" + "liiifipl" + "p"),
+    "pp_shared_prefix_attention_workspace_bytes": ("l", "p"), "pp_shared_prefix_attention": ("i", "pp"),
+}
+
 _lib = None
 
 
@@ -85,10 +97,11 @@ def lib():
     L.pp_last_error_string.restype = C.c_char_p
     for name in ("pp_conv2d", "pp_sparse_window_attention"):
         getattr(L, name).argtypes = [C.c_void_p, C.c_void_p]
-    for name in ("pp_group_norm_workspace_floats", "pp_linear_i8_weight_bytes", "pp_shared_prefix_attention_workspace_bytes"):
-        getattr(L, name).restype = C.c_int64
+    for name, (res, sig) in _TOKEN_OPS.items():
+        f = getattr(L, name)
+        f.restype, f.argtypes = _CTYPES[res], [_CTYPES[c] for c in sig]
     if (L.pp_sizeof_conv_args() != C.sizeof(ConvArgs) or L.pp_sizeof_attn_args() != C.sizeof(AttnArgs) or
-            L.pp_sizeof_prefix_attn_args() != C.sizeof(PrefixAttnArgs)):
+            L.pp_sizeof_prefix_attn_args() != C.sizeof(PrefixAttnArgs) or C.sizeof(PrefixAttnArgs) != _PREFIX_ATTN.size):
         raise RuntimeError("libpropainter_hip.so ABI mismatch with propainter_amd/hip.py (struct sizes differ)")
     _lib = L
     return L
@@ -757,154 +770,222 @@ def instance_norm_split(x, relu=False, eps=1e-5, residual=None, res_choff=0, rel
     return out
 
 
-def _same_device(who, x, *others):
+# ---- token operators: group norm, 8-bit linear layer, shared-prefix attention.  Their calls are short, so the host's share counts: argument
+# types are declared once (_TOKEN_OPS), sizes of workspaces remembered by shape, and nothing is wrapped unless somebody measures or checks.
+def _launch(what, cls, flops, nbytes, reads, writes, fn, *args):
+    if _profiler is None and not _FENCE_EVERY_LAUNCH and _hazard.active() is None:
+        rc = fn(*args)
+        if rc:
+            _check(rc, what)
+        return
+    for t in reads:
+        _p(t)
+    for t in writes:
+        _pw(t)
+    timed(cls, flops, nbytes, lambda: _check(fn(*args), what))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(who, x, *others):
+    """The current stream of x's device, which has to be the current device and everybody else's (see _stream)"""
+    require_gpu(x, who)
+    dev = x.get_device()
     for t in others:
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{who}: tensors on {x.device} and {t.device}")
+    if dev != torch._C._cuda_getDevice():
+        _stream(x)                                # raises
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+@functools.lru_cache(maxsize=4096)
+def _group_norm_floats(N, H, W, Cc, groups):
+    n = lib().pp_group_norm_workspace_floats(N, H, W, Cc, groups)
+    if n < 0:
+        raise ValueError(f"group_norm: map {H}x{W}, {Cc} channels (a multiple of 8, at most 2048), {groups} groups (must divide the channels)")
+    return n
 
 
 def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, act_param=0.0, out=None, x_choff=0, C_=None, out_choff=0):
     """GroupNorm + activation over channels [x_choff, x_choff + C_) of x NHWC [N,H,W,Cx] -> channels [out_choff, ..) of `out` (allocated
     [N,H,W,C_] if None; may be x itself with the same window).  gamma / beta fp32 [C_] or None; act: an ACT_* code (ACT_SILU included),
     act_param the slope of ACT_LRELU (pp_group_norm)."""
+    require_gpu(x, "group_norm")
     N, H, W, Cx = x.shape
     C_ = Cx - x_choff if C_ is None else C_
-    require_gpu(x, "group_norm")
     if out is None:
         out = torch.empty((N, H, W, C_), dtype=x.dtype, device=x.device)
-    _same_device("group_norm", x, gamma, beta, out)
-    assert x.is_contiguous() and out.is_contiguous() and out.dtype == x.dtype and out.shape[:3] == x.shape[:3]
-    for t in (gamma, beta):
-        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.shape == (C_,))
-    if out.data_ptr() == x.data_ptr() and (out.shape != x.shape or out_choff != x_choff):
-        raise ValueError("group_norm: in place needs the same channel window")
+    else:
+        assert out.is_contiguous() and out.dtype == x.dtype and out.shape[:3] == x.shape[:3]
+        if out.data_ptr() == x.data_ptr() and (out.shape != x.shape or out_choff != x_choff):
+            raise ValueError("group_norm: in place needs the same channel window")
+    stream = _raw_stream("group_norm", x, gamma, beta, out)
+    assert x.is_contiguous()
+    assert gamma is None or (gamma.dtype == torch.float32 and gamma.is_contiguous() and gamma.shape == (C_,))
+    assert beta is None or (beta.dtype == torch.float32 and beta.is_contiguous() and beta.shape == (C_,))
     if N == 0:
         return out
-    L = lib()
-    n = int(L.pp_group_norm_workspace_floats(_i(N), _i(H), _i(W), _i(C_), _i(groups)))
-    if n < 0:
-        raise ValueError(f"group_norm: map {H}x{W}, {C_} channels (a multiple of 8, at most 2048), {groups} groups (must divide the channels)")
-    ws = torch.empty((n,), dtype=torch.float32, device=x.device)
-    nb = N * H * W * C_ * x.element_size()
-    timed("group_norm", 0, 3 * nb, lambda: _check(L.pp_group_norm(_p(x), _i(Cx), _i(x_choff), _pw(out), _i(out.shape[-1]), _i(out_choff), _p(gamma), _p(beta),
-                                                                  _pw(ws), _i(N), _i(H), _i(W), _i(C_), _i(groups), C.c_float(eps), _i(act),
-                                                                  C.c_float(act_param), _i(dtype_code(x.dtype)), _stream(x)), "pp_group_norm"))
+    n = _group_norm_floats(N, H, W, C_, groups)
+    ws = torch.empty((n,), dtype=torch.float32, device=x.device) if n else None
+    _launch("pp_group_norm", "group_norm", 0, 3 * N * H * W * C_ * x.element_size(), (x, gamma, beta), (out, ws), lib().pp_group_norm, x.data_ptr(), Cx, x_choff,
+            out.data_ptr(), out.shape[3], out_choff, _ptr(gamma), _ptr(beta), _ptr(ws), N, H, W, C_, groups, eps, act, act_param, dtype_code(x.dtype), stream)
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def i8_row_bytes(K):
-    n = lib().pp_i8_row_bytes(_i(K))
+    n = lib().pp_i8_row_bytes(K)
     if n < 0:
         raise ValueError(f"8-bit rows hold 1 to 131072 values, not {K}")
     return n
+
+
+def _token_rows(who, x):
+    """(rows, K, elements between rows) of tokens [..., K] whose rows are one stride apart"""
+    K = x.shape[-1]
+    if x.dim() == 2:
+        rows, rs = x.shape[0], x.stride(0)
+    elif x.is_contiguous():
+        rows, rs = x.numel() // max(K, 1), K
+    else:
+        x2 = x.view(-1, K)                        # (raises where the rows are not one stride apart)
+        rows, rs = x2.shape[0], x2.stride(0)
+    if K > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{who}: the last dimension must be contiguous")
+    return rows, K, rs
 
 
 def quantize_tokens(x):
     """x [..., K] fp32 / fp16, rows any (one) stride apart -> (codes int8 [rows, K padded with zeros to a multiple of 64], scale fp32 [rows]):
     scale = max|row| / 127, code = row / scale rounded to the nearest integer, ties to even (pp_quantize_tokens).  Rows with a NaN or an
     infinity: scale NaN."""
-    require_gpu(x, "quantize_tokens")
-    K = x.shape[-1]
-    code = dtype_code(x.dtype)
-    Kp = i8_row_bytes(K)
-    rows = x.numel() // K
-    if K > 1 and x.stride(-1) != 1:
-        raise ValueError("quantize_tokens: the last dimension must be contiguous")
-    x2 = x.view(rows, K) if x.dim() != 2 else x            # (raises where the rows are not one stride apart)
+    stream = _raw_stream("quantize_tokens", x)
+    rows, K, rs = _token_rows("quantize_tokens", x)
+    code, Kp = dtype_code(x.dtype), i8_row_bytes(K)
     q = torch.empty((rows, Kp), dtype=torch.int8, device=x.device)
     scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
     if rows:
-        timed("quantize_tokens", 0, _nbytes(x) + _nbytes(q) + _nbytes(scale),
-              lambda: _check(lib().pp_quantize_tokens(_p(x2), C.c_int64(x2.stride(0) if rows > 1 else Kp), _pw(q), C.c_int64(Kp), _pw(scale), C.c_int64(rows), _i(K),
-                                                      _i(code), _stream(x)), "pp_quantize_tokens"))
+        _launch("pp_quantize_tokens", "quantize_tokens", 0, rows * (K * x.element_size() + Kp + 4), (x,), (q, scale), lib().pp_quantize_tokens, x.data_ptr(), rs,
+                q.data_ptr(), Kp, scale.data_ptr(), rows, K, code, stream)
     return q, scale
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_i8_bytes(N, K):
+    n = lib().pp_linear_i8_weight_bytes(N, K)
+    if n < 0:
+        raise ValueError(f"8-bit linear layer of {K} inputs and {N} outputs: 1 to 131072 inputs and 1 to 4194240 outputs")
+    return n
 
 
 def linear_i8_pack(wq, K=None):
     """Codes int8 [N, >= K] -> the weight layout of linear_i8 (pp_linear_i8_pack)."""
-    require_gpu(wq, "linear_i8_pack")
+    stream = _raw_stream("linear_i8_pack", wq)
     N = wq.shape[0]
     K = wq.shape[1] if K is None else K
     assert wq.dtype == torch.int8 and wq.dim() == 2 and wq.is_contiguous() and wq.shape[1] >= K
-    n = int(lib().pp_linear_i8_weight_bytes(_i(N), _i(K)))
-    if n < 0:
-        raise ValueError(f"8-bit linear layer of {K} inputs and {N} outputs: 1 to 131072 inputs and 1 to 4194240 outputs")
-    w = torch.empty((n,), dtype=torch.int8, device=wq.device)
-    _check(lib().pp_linear_i8_pack(_p(wq), C.c_int64(wq.shape[1]), _pw(w), _i(N), _i(K), _stream(wq)), "pp_linear_i8_pack")
+    w = torch.empty((_linear_i8_bytes(N, K),), dtype=torch.int8, device=wq.device)
+    _launch("pp_linear_i8_pack", "linear_i8_pack", 0, _nbytes(wq) + _nbytes(w), (wq,), (w,), lib().pp_linear_i8_pack, wq.data_ptr(), wq.shape[1], w.data_ptr(), N, K, stream)
     return w
+
+
+def _linear_i8_out(who, weight, wscale, bias, N, K, M, dtype, out, device):
+    assert wscale.dtype == torch.float32 and wscale.is_contiguous() and wscale.shape == (N,)
+    assert bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.shape == (N,))
+    assert weight.dtype == torch.int8 and weight.is_contiguous() and weight.numel() == _linear_i8_bytes(N, K)
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=device), N
+    if out.dim() != 2 or out.shape[0] != M or out.shape[1] < N or (M and (out.stride(1) != 1 or (M > 1 and out.stride(0) < N))):
+        raise ValueError(f"{who}: out must be [{M}, >= {N}] with contiguous rows")
+    return out, max(out.stride(0), N)
 
 
 def linear_i8(q, scale, weight, wscale, bias, N, K, act=ACT_NONE, act_param=0.0, out_dtype=torch.float16, out=None):
     """act(codes @ weight codes^T * scale * wscale + bias): q int8 [M, i8_row_bytes(K)], scale fp32 [M] (quantize_tokens), weight from
     linear_i8_pack, wscale / bias fp32 [N] -> out [M, N] of out_dtype (or the first N columns of a given `out` [M, >= N])."""
     require_gpu(q, "linear_i8")
-    M = q.shape[0]
-    if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous() or q.shape[1] != i8_row_bytes(K):
-        raise ValueError(f"linear_i8: codes must be int8 [M, {i8_row_bytes(K)}] as quantize_tokens returns them, got {q.dtype} {tuple(q.shape)}")
-    if scale.shape != (M,) or scale.dtype != torch.float32 or not scale.is_contiguous():
+    M, Kp = q.shape[0], i8_row_bytes(K)
+    if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous() or q.shape[1] != Kp:
+        raise ValueError(f"linear_i8: codes must be int8 [M, {Kp}] as quantize_tokens returns them, got {q.dtype} {tuple(q.shape)}")
+    if scale.dtype != torch.float32 or scale.shape != (M,) or not scale.is_contiguous():
         raise ValueError(f"linear_i8: scales must be float32 [{M}]")
-    for t in (wscale, bias):
-        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.shape == (N,))
-    assert weight.numel() == int(lib().pp_linear_i8_weight_bytes(_i(N), _i(K))) and weight.dtype == torch.int8 and weight.is_contiguous()
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=q.device)
-    if out.dim() != 2 or out.shape[0] != M or out.shape[1] < N or (M and out.stride(1) != 1):
-        raise ValueError(f"linear_i8: out must be [{M}, >= {N}] with contiguous rows")
-    _same_device("linear_i8", q, scale, weight, wscale, bias, out)
+    out, ors = _linear_i8_out("linear_i8", weight, wscale, bias, N, K, M, out_dtype, out, q.device)
+    stream = _raw_stream("linear_i8", q, scale, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
     if M:
-        timed("linear_i8", 2.0 * M * N * K, _nbytes(q) + _nbytes(weight) + M * N * out.element_size(),
-              lambda: _check(lib().pp_linear_i8(_p(q), C.c_int64(q.shape[1]), _p(scale), _p(weight), _p(wscale), _p(bias), _pw(out), C.c_int64(max(out.stride(0), N)),
-                                                C.c_int64(M), _i(N), _i(K), _i(act), C.c_float(act_param), _i(code), _stream(q)), "pp_linear_i8"))
+        _launch("pp_linear_i8", "linear_i8", 2.0 * M * N * K, M * Kp + weight.numel() + M * N * out.element_size(), (q, scale, weight, wscale, bias), (out,),
+                lib().pp_linear_i8, q.data_ptr(), Kp, scale.data_ptr(), weight.data_ptr(), wscale.data_ptr(), _ptr(bias), out.data_ptr(), ors, M, N, K, act, act_param,
+                code, stream)
     return out
+
+
+def linear_i8_tokens(x, weight, wscale, bias, N, act=ACT_NONE, act_param=0.0, out_dtype=None, out=None):
+    """quantize_tokens and linear_i8 in one call: x [..., K] fp32 / fp16 -> [rows, N] (pp_linear_i8_tokens)."""
+    require_gpu(x, "linear_i8_tokens")
+    M, K, rs = _token_rows("linear_i8_tokens", x)
+    xcode, Kp = dtype_code(x.dtype), i8_row_bytes(K)
+    out, ors = _linear_i8_out("linear_i8_tokens", weight, wscale, bias, N, K, M, out_dtype or x.dtype, out, x.device)
+    stream = _raw_stream("linear_i8_tokens", x, weight, wscale, bias, out)
+    code = dtype_code(out.dtype)
+    if M:
+        need = lib().pp_linear_i8_tokens_workspace_bytes(M, K)
+        work = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+        _launch("pp_linear_i8_tokens", "linear_i8", 2.0 * M * N * K, M * K * x.element_size() + weight.numel() + M * N * out.element_size(), (x, weight, wscale, bias),
+                (out, work), lib().pp_linear_i8_tokens, x.data_ptr(), rs, xcode, weight.data_ptr(), wscale.data_ptr(), _ptr(bias), out.data_ptr(), ors, M, N, K, act,
+                act_param, code, _ptr(work), need, stream)
+    return out
+
+
+_PREFIX_ATTN = struct.Struct("@10if" + "Q3q" * 6 + "3Qq")      # PrefixAttnArgs, packed in one call
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_attn_bytes(*sizes):
+    """scratch of a call with these sizes (dtype, B, G, Lq, Hq, Hkv, D, P, S)"""
+    n = lib().pp_shared_prefix_attention_workspace_bytes(_PREFIX_ATTN.pack(*sizes, 0, 1.0, *(0,) * 28))
+    if n < 0:
+        raise ValueError(lib().pp_last_error_string().decode(errors="replace"))
+    return n
 
 
 def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal=False, scale=None, out=None):
     """softmax(scale * q K^T) V per sequence over the keys of a prefix that the B / G sequences of a group share and their own suffix keys:
     q [B,Lq,Hq,D]; pk / pv [G,P,Hkv,D] or None; k / v [B,S,Hkv,D] or None; Hq a multiple of Hkv, D 64 or 128, fp16 or fp32, any strides with a
     contiguous last dimension.  Sequence b belongs to group b // (B // G).  prefix_lens int32 [G] / lens int32 [B] (device): the keys that
-    count (default: all); causal: query i sees suffix keys up to lens[b] - Lq + i.  scale: default 1 / sqrt(D).  A query without keys gives
-    zeros.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
+    count (default: all); causal: query i sees suffix keys up to lens[b] - Lq + i, and the values that causality hides from a query have to
+    be finite.  scale: default 1 / sqrt(D).  A query without keys gives zeros.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
     require_gpu(q, "shared_prefix_attention")
-    B, Lq, Hq, D = q.shape
+    B, Lq, Hq, D = qshape = q.shape
+    dt = q.dtype
     if (pk is None) != (pv is None) or (k is None) != (v is None):
         raise ValueError("shared_prefix_attention: keys and values come together")
-    a = PrefixAttnArgs()
-    a.dtype, a.B, a.Lq, a.Hq, a.D = dtype_code(q.dtype), B, Lq, Hq, D
-    a.G, a.P = (pk.shape[0], pk.shape[1]) if pk is not None else (1, 0)
-    a.S = k.shape[1] if k is not None else 0
-    a.Hkv = pk.shape[2] if pk is not None else (k.shape[2] if k is not None else Hq)
+    G, P, Hkv = pk.shape[:3] if pk is not None else (1, 0, k.shape[2] if k is not None else Hq)
+    S = k.shape[1] if k is not None else 0
     if out is None:
-        out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    _same_device("shared_prefix_attention", q, pk, pv, k, v, prefix_lens, lens, out)
-    for name, t, shape in (("q", q, (B, Lq, Hq, D)), ("pk", pk, (a.G, a.P, a.Hkv, D)), ("pv", pv, (a.G, a.P, a.Hkv, D)), ("k", k, (B, a.S, a.Hkv, D)),
-                           ("v", v, (B, a.S, a.Hkv, D)), ("out", out, (B, Lq, Hq, D))):
+        out = torch.empty(qshape, dtype=dt, device=q.device)
+    stream = _raw_stream("shared_prefix_attention", q, pk, pv, k, v, prefix_lens, lens, out)
+    pshape, kshape = (G, P, Hkv, D), (B, S, Hkv, D)
+    packed = []
+    for name, t, shape in (("q", q, qshape), ("pk", pk, pshape), ("pv", pv, pshape), ("k", k, kshape), ("v", v, kshape), ("out", out, qshape)):
         if t is None:
+            packed += (0, 0, 0, 0)
             continue
-        if tuple(t.shape) != shape or t.dtype != q.dtype or (t.numel() and t.stride(3) != 1):
-            raise ValueError(f"shared_prefix_attention: {name} is {t.dtype} {tuple(t.shape)}, expected {q.dtype} {shape} with a contiguous last dimension")
-        setattr(a, name, t.data_ptr())
-        getattr(a, name + "_stride")[:] = t.stride()[:3]
-    for name, t, n in (("prefix_lens", prefix_lens, a.G), ("lens", lens, B)):
-        if t is not None:
-            if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
-                raise ValueError(f"shared_prefix_attention: {name} must be int32 [{n}]")
-            setattr(a, name, t.data_ptr())
-    a.causal, a.scale = int(bool(causal)), float(scale) if scale is not None else D ** -0.5
-    need = int(lib().pp_shared_prefix_attention_workspace_bytes(C.byref(a)))
-    if need < 0:
-        _check(need, "pp_shared_prefix_attention")
+        st = t.stride()
+        if t.shape != shape or t.dtype != dt or (st[3] != 1 and t.numel()):
+            raise ValueError(f"shared_prefix_attention: {name} is {t.dtype} {tuple(t.shape)}, expected {dt} {tuple(shape)} with a contiguous last dimension")
+        packed += (t.data_ptr(), st[0], st[1], st[2])
+    for name, t, n in (("prefix_lens", prefix_lens, G), ("lens", lens, B)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"shared_prefix_attention: {name} must be int32 [{n}]")
+    sizes = (dtype_code(dt), B, G, Lq, Hq, Hkv, D, P, S)
+    need = _prefix_attn_bytes(*sizes)
     work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-    if work is not None:
-        a.work, a.work_bytes = work.data_ptr(), need
-    for t in (q, pk, pv, k, v, prefix_lens, lens):
-        _p(t)
-    for t in (out, work):
-        _pw(t)
-    esz = q.element_size()
-    nb = esz * D * (2 * B * Lq * Hq + 2 * a.Hkv * (a.G * a.P + B * a.S))
-    timed("shared_prefix_attention", 4.0 * D * Hq * B * Lq * (a.P + a.S), nb,
-          lambda: _check(lib().pp_shared_prefix_attention(C.byref(a), _stream(q)), "pp_shared_prefix_attention"))
+    args = _PREFIX_ATTN.pack(*sizes, 1 if causal else 0, D ** -0.5 if scale is None else scale, *packed, _ptr(prefix_lens) or 0, _ptr(lens) or 0, _ptr(work) or 0, need)
+    _launch("pp_shared_prefix_attention", "shared_prefix_attention", 4.0 * D * Hq * B * Lq * (P + S), q.element_size() * D * (2 * B * Lq * Hq + 2 * Hkv * (G * P + B * S)),
+            (q, pk, pv, k, v, prefix_lens, lens), (out, work), lib().pp_shared_prefix_attention, args, stream)
     return out
 
 

@@ -127,7 +127,9 @@ def layer_of(conv, N, K, seed, bias=True):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 4096, 512), (2, 100, 30), (3, 1960, 512), (5, 512, 17), (16, 512, 1536), (17, 640, 100), (31, 65, 64), (32, 256, 257), (45, 512, 1536),
          (64, 1000, 65), (65, 128, 48), (100, 192, 1000), (127, 512, 130), (129, 320, 200), (200, 2048, 384), (256, 256, 256), (257, 300, 511), (333, 4100, 72), (513, 576, 640),
-         (1025, 64, 24), (2500, 200, 264), (300, 16384, 16)]
+         (1025, 64, 24), (2500, 200, 264), (300, 16384, 16), (20, 130, 9000), (1100, 1000, 1030)]
+# weights kept in registers (K <= 256, K <= 512, odd channel blocks), 128 x 256 tiles, 256 x 256 tiles
+LARGE = [(49200, 200, 200), (17000, 500, 1000), (50000, 65, 70), (25001, 512, 520), (4200, 600, 2100), (8200, 1960, 770), (8100, 6200, 4100)]
 
 
 @pytest.mark.parametrize("odt", [torch.float32, torch.float16])
@@ -141,8 +143,18 @@ def test_product(hip, conv, M, K, N, odt):
     assert torch.equal(got, layer.product(q, s, out_dtype=odt)), "two runs differ"
 
 
+@pytest.mark.parametrize("M,K,N", LARGE)
+def test_large_products(hip, conv, M, K, N):
+    layer, wq, ws, b = layer_of(conv, N, K, M + K + N)
+    q, s = hip.quantize_tokens(rand((M, K), torch.float16, M))
+    for odt in (torch.float16, torch.float32):
+        got = layer.product(q, s, act="relu", out_dtype=odt)
+        for a in range(0, M, 8192):
+            check(got[a:a + 8192], *reference(q[a:a + 8192, :K], s[a:a + 8192], wq, ws, b, "relu"))
+
+
 @pytest.mark.parametrize("dtype,odt", [(torch.float16, torch.float16), (torch.float32, torch.float16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32)])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (1, 4097, 70), (2, 4096, 33), (1, 8192, 64), (3, 64, 64), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32)])
 def test_layer_on_float_tokens(hip, conv, M, K, N, dtype, odt):
     layer, wq, ws, b = layer_of(conv, N, K, 5)
     x = rand((M, K), dtype, 6)
