@@ -124,6 +124,24 @@ __device__ __forceinline__ float act_value(float v, int act, float param) {
   }
 }
 
+// The same for N values: one decision for all of them (a decision a value cost more than the values' own arithmetic)
+template <int N> __device__ __forceinline__ void act_values(float* v, int act, float param) {
+#define PP_ACT_EACH(code)                                       \
+  case code:                                                    \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = act_value(v[i], code, param); \
+    break;
+  switch (act) {
+    PP_ACT_EACH(PP_ACT_RELU)
+    PP_ACT_EACH(PP_ACT_LRELU)
+    PP_ACT_EACH(PP_ACT_SIGMOID)
+    PP_ACT_EACH(PP_ACT_TANH)
+    PP_ACT_EACH(PP_ACT_GELU)
+    PP_ACT_EACH(PP_ACT_SILU)
+    default: break;
+  }
+#undef PP_ACT_EACH
+}
+
 // Loads `n` (<= 8) consecutive elements as fp32.
 template <typename T> __device__ __forceinline__ void load8(const T* p, float* v) {
   if constexpr (sizeof(T) == 2) {

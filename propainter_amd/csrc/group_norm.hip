@@ -6,6 +6,7 @@
 // Statistics are held in fp32 as (count, mean, sum of squared deviations) and joined pairwise (Chan et al. 1979): no difference of large
 // sums of squares, so a map whose mean is far from zero loses nothing.  The order of every sum is fixed by the sizes: no atomics.
 #include "common.h"
+#include "attn_lanes.h"
 
 namespace pp {
 
@@ -94,8 +95,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   __shared__ float gm[2048], gr[2048];                 // mean and rstd of every group (groups <= C <= 2048)
   __shared__ float part_n[256], part_m[256], part_v[256];
-  // images and pixels in the opposite order of the statistics: what was read last is still in the cache
-  const int t = threadIdx.x, n = gridDim.y - 1 - blockIdx.y;
+  const int t = threadIdx.x, n = blockIdx.y;
   const float* part = p.part + (long long)n * p.slices * p.groups * 2;
   const int per = p.groups < 256 ? 256 / p.groups : 1;  // threads that share one group's slices
   for (int g0 = 0; g0 < p.groups; g0 += 256) {
@@ -137,8 +137,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   }
   const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + col * 8;
   T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + col * 8;
-  const long long q0 = (long long)(gridDim.x - 1 - blockIdx.x) * p.ppblock, q1 = min(q0 + p.ppblock, (long long)p.HW);
-  constexpr int U = 4;                                  // loads in flight a thread
+  const long long q0 = (long long)blockIdx.x * p.ppblock, q1 = min(q0 + p.ppblock, (long long)p.HW);
+  constexpr int U = 2;                                  // loads in flight a thread (1: 77.5 us, 2: 78.5 / 66.0, 4: 86.4 / 69.9 at 4x360x640x64 fp16 / 2x270x480x96 fp32)
   for (long long q = q0 + pr; q < q1; q += U * rows) {
     float v[U][8];
 #pragma unroll
@@ -148,7 +148,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
     for (int u = 0; u < U; ++u)
       if (q + u * rows < q1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = act_value(fmaf(v[u][i] - mean[i], mul[i], add[i]), p.act, p.act_param);
+        for (int i = 0; i < 8; ++i) v[u][i] = fmaf(v[u][i] - mean[i], mul[i], add[i]);
+        act_values<8>(v[u], p.act, p.act_param);
         store8<T>(y + (q + u * rows) * p.out_cs, v[u]);
       }
   }
@@ -157,8 +158,13 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
 // Sum over the block, the same value in every thread; two barriers.
 template <int BLOCK>
 __device__ __forceinline__ float block_sum(float v, float* lds) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+#if defined(__HIP_DEVICE_COMPILE__)
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, false));      // rotations inside 16 lanes: 8, 4, 2, 1
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x124, 0xf, 0xf, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x122, 0xf, 0xf, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x121, 0xf, 0xf, false));
+  v = rows_sum(v);
+#endif
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0.f;
@@ -169,67 +175,68 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
 }
 
 // A group that fits a block's registers (channels of a group a multiple of 8): one launch, one read; the variance is a second pass over registers.
+// A thread keeps one column of 8 channels and walks the pixels.
 constexpr int GN_VEC = 8;         // vectors of 8 a thread
 template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void gn_group_kernel(const GnParams p) {
-  __shared__ float red[BLOCK / 64];
-  const int g = blockIdx.x, n = blockIdx.y, vpp = p.cg >> 3, total = p.HW * vpp;
-  const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + g * p.cg;
-  T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + g * p.cg;
-  float v[GN_VEC][8];
+  __shared__ float red[2][BLOCK / 64];
+  const int g = blockIdx.x, n = blockIdx.y, vpp = p.cg >> 3, rows = BLOCK / vpp;
+  const int pr = (int)threadIdx.x / vpp, c = ((int)threadIdx.x - pr * vpp) * 8;
+  const int last = pr < rows ? p.HW : 0;            // threads past the last whole row of columns have no pixels
+  const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + g * p.cg + c;
+  T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + g * p.cg + c;
+  float v[GN_VEC][8], gm[8], bt[8];
+#pragma unroll
+  for (int k = 0; k < GN_VEC; ++k)
+    if (pr + k * rows < last) load8<T>(x + (pr + k * rows) * p.in_cs, v[k]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    gm[j] = p.gamma != nullptr ? p.gamma[g * p.cg + c + j] : 1.f;
+    bt[j] = p.beta != nullptr ? p.beta[g * p.cg + c + j] : 0.f;
+  }
   float sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < GN_VEC; ++k) {
-    const int i = k * BLOCK + threadIdx.x, px = i / vpp;
-    if (i < total) {
-      load8<T>(x + px * p.in_cs + (i - px * vpp) * 8, v[k]);
+  for (int k = 0; k < GN_VEC; ++k)
+    if (pr + k * rows < last) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += v[k][j];
     }
-  }
   const float count = (float)p.HW * (float)p.cg;
-  const float mean = block_sum<BLOCK>(sum, red) / count;
+  const float mean = block_sum<BLOCK>(sum, red[0]) / count;
   float dev = 0.f;
 #pragma unroll
   for (int k = 0; k < GN_VEC; ++k)
-    if (k * BLOCK + (int)threadIdx.x < total) {
+    if (pr + k * rows < last) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[k][j] -= mean;
         dev = fmaf(v[k][j], v[k][j], dev);
       }
     }
-  const float rstd = 1.f / sqrtf(block_sum<BLOCK>(dev, red) / count + p.eps);
+  const float rstd = 1.f / sqrtf(block_sum<BLOCK>(dev, red[1]) / count + p.eps);
 #pragma unroll
-  for (int k = 0; k < GN_VEC; ++k) {
-    const int i = k * BLOCK + threadIdx.x, px = i / vpp;
-    if (i < total) {
-      const int c = (i - px * vpp) * 8;
-      float gm[8], bt[8];
+  for (int j = 0; j < 8; ++j) gm[j] *= rstd;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { gm[j] = rstd; bt[j] = 0.f; }
-      if (p.gamma != nullptr)
+  for (int k = 0; k < GN_VEC; ++k)
+    if (pr + k * rows < last) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gm[j] = rstd * p.gamma[g * p.cg + c + j];
-      if (p.beta != nullptr)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bt[j] = p.beta[g * p.cg + c + j];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = act_value(fmaf(v[k][j], gm[j], bt[j]), p.act, p.act_param);
-      store8<T>(y + px * p.out_cs + c, v[k]);
+      for (int j = 0; j < 8; ++j) v[k][j] = fmaf(v[k][j], gm[j], bt[j]);
+      act_values<8>(v[k], p.act, p.act_param);
+      store8<T>(y + (pr + k * rows) * p.out_cs, v[k]);
     }
-  }
 }
 
 }  // namespace pp
 
 using namespace pp;
 
-// A group in one block's registers: its share of a map is small, or there are groups enough to fill the chip.  Measured in one launch against two:
-// 30 x 54 x 128 in 8 groups FIGURE.
-static bool gn_in_registers(int64_t HW, int C, int groups) {
+// A group in one block's registers where it fits: 30 x 54 x 128 in 8 groups ONEFIG us in one launch, 11.7 in two.
+static int gn_group_block(int64_t HW, int C, int groups) {      // threads, 0: it does not fit
   const int cg = C / groups;
-  return cg % 8 == 0 && HW * cg <= 1024 * GN_VEC * 8;
+  if (cg % 8 != 0) return 0;
+  for (int block = 256; block <= 1024; block *= 2)
+    if (cg / 8 <= block && HW <= (int64_t)GN_VEC * (block / (cg / 8))) return block;
+  return 0;
 }
 
 static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
@@ -245,7 +252,7 @@ static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
 
 extern "C" int64_t pp_group_norm_workspace_floats(int N, int H, int W, int C, int groups) {
   if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 != 0 || C > 2048 || groups <= 0 || C % groups != 0 || (int64_t)H * W > 0x7fffffff) return PP_ERR_ARG;
-  if (gn_in_registers((int64_t)H * W, C, groups)) return 0;
+  if (gn_group_block((int64_t)H * W, C, groups)) return 0;
   int slices, pps;
   gn_split(N, H * W, C, &slices, &pps);
   return (int64_t)N * slices * groups * 2;
@@ -267,7 +274,7 @@ extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void*
                  (uintptr_t)stats_ws % 8 == 0,
              PP_ERR_ALIGN, "pp_group_norm: strides and channel offsets must be multiples of 8, the buffers 16-byte aligned");
   const int HW = H * W;
-  const bool one = gn_in_registers(HW, C, groups);
+  const int one = gn_group_block(HW, C, groups);
   PP_REQUIRE(one || stats_ws, PP_ERR_WORKSPACE, "pp_group_norm: needs %lld floats of scratch", (long long)pp_group_norm_workspace_floats(N, H, W, C, groups));
   GnParams p;
   p.in = (const char*)in; p.out = (char*)out; p.gamma = gamma; p.beta = beta; p.part = stats_ws;
@@ -276,14 +283,13 @@ extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void*
   hipStream_t st = (hipStream_t)stream;
   if (one) {
     const dim3 grid(groups, N);
-    const bool small = (int64_t)HW * p.cg <= 256 * GN_VEC * 8;
-    if (dtype == PP_F16) {
-      if (small) hipLaunchKernelGGL((gn_group_kernel<_Float16, 256>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((gn_group_kernel<_Float16, 1024>), grid, dim3(1024), 0, st, p);
-    } else {
-      if (small) hipLaunchKernelGGL((gn_group_kernel<float, 256>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((gn_group_kernel<float, 1024>), grid, dim3(1024), 0, st, p);
-    }
+#define PP_GN_GROUP(T)                                                                                \
+  if (one == 256) hipLaunchKernelGGL((gn_group_kernel<T, 256>), grid, dim3(256), 0, st, p);           \
+  else if (one == 512) hipLaunchKernelGGL((gn_group_kernel<T, 512>), grid, dim3(512), 0, st, p);      \
+  else hipLaunchKernelGGL((gn_group_kernel<T, 1024>), grid, dim3(1024), 0, st, p)
+    if (dtype == PP_F16) { PP_GN_GROUP(_Float16); }
+    else { PP_GN_GROUP(float); }
+#undef PP_GN_GROUP
     return launch_status("pp_group_norm");
   }
   gn_split(N, HW, C, &p.slices, &p.ppslice);

@@ -299,10 +299,7 @@ template <typename TO> struct Lane8 {
   __device__ __forceinline__ void value(const LinI8Params& p, float xs, const i32x4* acc, float* v) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = fmaf((float)acc[i >> 2][i & 3] * xs, ws[i], bias[i]);
-    if (p.act != PP_ACT_NONE) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], p.act, p.act_param);
-    }
+    act_values<8>(v, p.act, p.act_param);
   }
   __device__ __forceinline__ void store(const LinI8Params& p, long long m, const float* v) const {
     TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c;
