@@ -23,20 +23,36 @@ struct PaPart {
   int nper;              // sequences a row space packs (1 or nseq)
   int rows, rowblocks;   // rows of a space, blocks that cover them
   int prefix, suffix;    // keys it walks
-  int nsplit, slot0;     // key splits; first scratch slot
+  int items, whole;      // row blocks over all spaces and key heads; the first `whole` walk all their keys and write the output
+  int nsplit, slot0;     // the others: blocks that share the keys; first scratch slot
+  int by_row;            // scratch rows: 1 = query rows of the call (two parts join there), 0 = rows of the split items alone
+  int blocks;            // whole + (items - whole) * nsplit
 };
 struct PaParams {
   const char *q, *pk, *pv, *k, *v;
   char* out;
   const int *plens, *lens;
-  float* part_o;         // [slots][B * Lq * Hq][D], NULL: one split writes the output itself
-  float* part_ml;        // [slots][B * Lq * Hq][2]
+  float* part_o;         // scratch [slots][prows][D]: unnormalised outputs
+  float* part_ml;        // scratch [slots][prows][2]: maximum and sum
+  long long prows;
   long long qs[3], pks[3], pvs[3], ks[3], vs[3], os[3];
   int B, G, nseq, Lq, Hq, Hkv, rep, P, S, causal, slots;
   float sc2;             // |scale| * log2(e)  (1 if scale is 0)
   float qsign;           // sign of scale (0 if it is 0), taken into the queries
-  PaPart part;
+  PaPart part[2];
 };
+
+// blocks 8 apart share an XCD: give each XCD one contiguous run of 0 .. n - 1, so that blocks that read the same keys meet in one L2
+__device__ __forceinline__ int xcd_run(int id, int n) {
+  const int per = n >> 3, extra = n & 7, x = id & 7;
+  return x * per + min(x, extra) + (id >> 3);
+}
+// query row r of row space `space` and key head hk -> sequence, token, head
+struct PaRow { int b, i, h; };
+__device__ __forceinline__ PaRow pa_row(int Lq, int rep, int nper, int space, int hk, int r) {
+  const int rpseq = Lq * rep, sq = r / rpseq, rest = r - sq * rpseq, i = rest / rep;
+  return {space * nper + sq, i, hk * rep + (rest - i * rep)};
+}
 
 constexpr float PA_NONE = -3.4028235e38f;   // running maximum before the first key: finite, so that masked scores (-inf) weigh 0
 
@@ -72,33 +88,44 @@ template <typename T, int D, bool WK> struct PaTile {
   static constexpr int KBYTES = KT * D * (int)sizeof(T), VBYTES = KT * VLD * (int)sizeof(T);
 };
 
+template <typename T, int D, int QT, bool WK> struct PaLds {
+  typedef PaTile<T, D, WK> C;
+  static constexpr int JOIN = WK ? 4 * 16 * QT * (D + 4) * 4 : 0;
+  static constexpr int BYTES = C::KBYTES + C::VBYTES > JOIN ? C::KBYTES + C::VBYTES : JOIN;
+};
+
+// block `bid` of part `pt`
 template <typename T, int D, int QT, bool WK>
-__global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
+__device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, const int bid, char* lds, float* wave_ml) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef PaTile<T, D, WK> C;
   typedef typename PaOps<T>::frag frag;
   constexpr int KT = C::KT, NK = C::NK, STEPS = C::STEPS, DT = D / 16;
-  constexpr int JOIN = WK ? 4 * 16 * QT * (D + 4) * 4 : 0;
-  constexpr int LDS = C::KBYTES + C::VBYTES > JOIN ? C::KBYTES + C::VBYTES : JOIN;
-  __shared__ __attribute__((aligned(16))) char lds[LDS];
-  __shared__ float wave_ml[WK ? 4 * 16 * QT * 2 : 1];
   T* Ks = reinterpret_cast<T*>(lds);
   T* Vs = reinterpret_cast<T*>(lds + C::KBYTES);
-  const PaPart& pt = p.part;
 
-  // ---- block -> (row block fastest, split, key head, row space); blocks 8 apart share an XCD: each XCD gets one contiguous run, so that
-  // the row blocks that read the same keys meet in one L2
-  long long id = blockIdx.x;
-  {
-    const long long n = gridDim.x, per = n >> 3, extra = n & 7, x = id & 7;
-    id = x * per + (x < extra ? x : extra) + (id >> 3);
+  // ---- block -> item (row block fastest, key head, row space) and key split
+  int item, split = 0;
+  const bool whole = bid < pt.whole;
+  if (whole) {
+    item = xcd_run(bid, pt.whole);
+  } else {
+    const int x = xcd_run(bid - pt.whole, pt.blocks - pt.whole), rest = pt.items - pt.whole;
+    // row blocks of one space and split are neighbours where they all are split
+    if (pt.whole == 0) {
+      const int rb = x % pt.rowblocks, y = x / pt.rowblocks;
+      split = y % pt.nsplit;
+      item = y / pt.nsplit * pt.rowblocks + rb;
+    } else {
+      split = x / rest;
+      item = pt.whole + x % rest;
+    }
   }
-  const int rb = (int)(id % pt.rowblocks); id /= pt.rowblocks;
-  const int split = (int)(id % pt.nsplit); id /= pt.nsplit;
-  const int hk = (int)(id % p.Hkv);
-  const int space = (int)(id / p.Hkv);
+  const int nsplit = whole ? 1 : pt.nsplit;
+  const int rb = item % pt.rowblocks;
+  const int hk = item / pt.rowblocks % p.Hkv;
+  const int space = item / pt.rowblocks / p.Hkv;
   const int b0 = space * pt.nper, g = b0 / p.nseq;
-  const int rpseq = p.Lq * p.rep;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lg = lane >> 4, lc = lane & 15;
   const int row0 = rb * 16 * QT * (WK ? 1 : 4);
   const int row_end = min(pt.rows, row0 + 16 * QT * (WK ? 1 : 4));
@@ -112,7 +139,7 @@ __global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
   }
   const int ptiles = (np + KT - 1) / KT;
   const int tiles = ptiles + (vis_max + KT - 1) / KT;
-  const int t0 = (int)((long long)tiles * split / pt.nsplit), t1 = (int)((long long)tiles * (split + 1) / pt.nsplit);
+  const int t0 = (int)((long long)tiles * split / nsplit), t1 = (int)((long long)tiles * (split + 1) / nsplit);
 
   // ---- this lane's queries (column lane & 15 of the wave's row tiles)
   frag qf[QT][STEPS];
@@ -121,16 +148,15 @@ __global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
   char* optr[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    const int r = row0 + (WK ? qt : wave * QT + qt) * 16 + lc;
+    const int rl = (WK ? qt : wave * QT + qt) * 16 + lc, r = row0 + rl;
     const bool ok = r < pt.rows;
-    const int rr = ok ? r : 0;
-    const int sq = rr / rpseq, rest = rr - sq * rpseq;
-    const int i = rest / p.rep, h = hk * p.rep + (rest - i * p.rep);
-    const int b = b0 + sq;
-    rowid[qt] = ok ? ((long long)b * p.Lq + i) * p.Hq + h : -1;
-    vis[qt] = p.causal ? max(0, ns - p.Lq + i + 1) : ns;
-    optr[qt] = p.out + (b * p.os[0] + i * p.os[1] + h * p.os[2]) * (long long)sizeof(T);
-    const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+    const PaRow w = pa_row(p.Lq, p.rep, pt.nper, space, hk, ok ? r : 0);
+    // row of the scratch (-1: no row)
+    rowid[qt] = !ok ? -1 : pt.by_row ? ((long long)w.b * p.Lq + w.i) * p.Hq + w.h : (long long)(item - pt.whole) * (16 * QT * (WK ? 1 : 4)) + rl;
+    if (ok && whole) rowid[qt] = 0;
+    vis[qt] = p.causal ? max(0, ns - p.Lq + w.i + 1) : ns;
+    optr[qt] = p.out + (w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2]) * (long long)sizeof(T);
+    const T* qp = reinterpret_cast<const T*>(p.q) + w.b * p.qs[0] + w.i * p.qs[1] + w.h * p.qs[2];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       frag f = *reinterpret_cast<const frag*>(qp + (s * 4 + lg) * (16 / sizeof(T)));
@@ -291,8 +317,8 @@ __global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
     for (int qt = 0; qt < QT; ++qt) {
       const float l = rows_sum(l_run[qt]);
       if (rowid[qt] < 0) continue;
-      if (p.part_o != nullptr) {
-        const long long at = (pt.slot0 + split) * ((long long)p.B * p.Lq * p.Hq) + rowid[qt];
+      if (!whole) {
+        const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
         if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_run[qt], l);
         if (t0 < t1) {
 #pragma unroll
@@ -351,14 +377,14 @@ __global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
       const float* e = jo + (qt * 16 + lc) * JLD + c0;
       constexpr int W = 16 * QT * JLD;
       const float inv = lj[qt] != 0.f ? 1.f / lj[qt] : 0.f;
-      const long long at = (pt.slot0 + split) * ((long long)p.B * p.Lq * p.Hq) + rowid[qt];
-      if (p.part_o != nullptr && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
+      const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
+      if (!whole && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
 #pragma unroll
       for (int c = 0; c < D / 16; c += 4) {
         f32x4 v = *reinterpret_cast<const f32x4*>(e + c);
 #pragma unroll
         for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + c);
-        if (p.part_o != nullptr) {
+        if (!whole) {
           if (t0 < t1) *reinterpret_cast<f32x4*>(p.part_o + at * D + c0 + c) = v;
         } else if constexpr (C::F16) {
           const f16x4 o = {(_Float16)(v[0] * inv), (_Float16)(v[1] * inv), (_Float16)(v[2] * inv), (_Float16)(v[3] * inv)};
@@ -372,39 +398,75 @@ __global__ __launch_bounds__(256, 1) void pa_tile_kernel(const PaParams p) {
 #endif
 }
 
-// One wave per row: the slots' outputs, weighted by exp2(max - common max), over the weighted sum.  A slot without keys (sum 0) left no output.
+// One part a launch, or the two parts of a call in one, the packed rows' products (part 1) first: they run next to the memory-bound walks of the
+// suffixes (part 0).
+// waves a SIMD the registers are to allow: two blocks a CU, but for fp32 heads of 128 in two row tiles, which do not fit
+template <typename T, int D, int QT> constexpr int pa_waves() { return sizeof(T) == 4 && D == 128 && QT == 2 ? 1 : 2; }
+
+template <typename T, int D, int QT, bool WK>
+__global__ __launch_bounds__(256, (pa_waves<T, D, QT>())) void pa_tile_kernel(const PaParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[PaLds<T, D, QT, WK>::BYTES];
+  __shared__ float wave_ml[WK ? 4 * 16 * QT * 2 : 1];
+  pa_block<T, D, QT, WK>(p, p.part[0], (int)blockIdx.x, lds, wave_ml);
+}
+template <typename T, int D, int QT0, bool WK0, int QT1, bool WK1>
+__global__ __launch_bounds__(256, (pa_waves<T, D, (QT0 > QT1 ? QT0 : QT1)>())) void pa_pair_kernel(const PaParams p) {
+  constexpr int B0 = PaLds<T, D, QT0, WK0>::BYTES, B1 = PaLds<T, D, QT1, WK1>::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[B0 > B1 ? B0 : B1];
+  __shared__ float wave_ml[4 * 16 * 2 * 2];
+  if ((int)blockIdx.x < p.part[1].blocks) pa_block<T, D, QT1, WK1>(p, p.part[1], (int)blockIdx.x, lds, wave_ml);
+  else pa_block<T, D, QT0, WK0>(p, p.part[0], (int)blockIdx.x - p.part[1].blocks, lds, wave_ml);
+}
+
+// One wave per split row: the slots' outputs, weighted by exp2(max - common max), over the weighted sum.  A slot without keys (sum 0) left no output:
+// what the scratch holds there is read and dropped.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p) {
+__global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p, const int per) {
   const int lane = threadIdx.x & 63;
-  const long long rows = (long long)p.B * p.Lq * p.Hq;
   const long long row = blockIdx.x * 4ll + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  constexpr int E = D / 64;
+  if (row >= p.prows) return;
+  const PaPart& pt = p.part[0];
+  PaRow w;
+  if (pt.by_row) {
+    w = {(int)(row / p.Hq / p.Lq), (int)(row / p.Hq % p.Lq), (int)(row % p.Hq)};
+  } else {
+    const int item = pt.whole + (int)(row / per), rb = item % pt.rowblocks, r = rb * per + (int)(row % per);
+    if (r >= pt.rows) return;
+    w = pa_row(p.Lq, p.rep, pt.nper, item / pt.rowblocks / p.Hkv, item / pt.rowblocks % p.Hkv, r);
+  }
+  constexpr int E = D / 64, U = 8;
   float m = PA_NONE, l = 0.f;                      // slots <= 64: one a lane
   if (lane < p.slots) {
-    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + (lane * rows + row) * 2);
+    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + (lane * p.prows + row) * 2);
     m = e.x;
     l = e.y;
   }
   float mj = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mj = fmaxf(mj, __shfl_xor(mj, o));
-  const float w = l != 0.f ? __builtin_amdgcn_exp2f(m - mj) : 0.f;
-  float total = l * w;
+  const float wt = l != 0.f ? __builtin_amdgcn_exp2f(m - mj) : 0.f;
+  float total = l != 0.f ? l * wt : 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < p.slots; ++s) {
-    const float ls = __shfl(l, s), ws = __shfl(w, s);
-    if (ls != 0.f) {                               // (a NaN sum is not 0: its output is read and stays NaN)
+  const float* src = p.part_o + row * D + lane * E;
+  for (int s0 = 0; s0 < p.slots; s0 += U) {
+    float v[U][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p.part_o[(s * rows + row) * D + lane * E + e], acc[e]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[u][e] = src[(long long)min(s0 + u, p.slots - 1) * p.prows * D + e];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int sl = min(s0 + u, 63);
+      const float ls = __shfl(l, sl), ws = __shfl(wt, sl);       // (lanes past the last slot: sum 0; a NaN sum is not 0 and stays)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = s0 + u < p.slots && ls != 0.f ? fmaf(ws, v[u][e], acc[e]) : acc[e];
     }
   }
-  const int h = (int)(row % p.Hq), i = (int)(row / p.Hq % p.Lq), b = (int)(row / p.Hq / p.Lq);
-  T* o = reinterpret_cast<T*>(p.out) + b * p.os[0] + i * p.os[1] + h * p.os[2] + lane * E;
+  T* o = reinterpret_cast<T*>(p.out) + w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2] + lane * E;
   const float inv = total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
@@ -413,63 +475,90 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p) {
 // ---- the plan of a call: which parts, which tile form, how many key splits.  A function of sizes and types alone (lengths stay on the device).
 struct PaPlan {
   int nparts, slots;
+  long long prows;       // rows of the scratch
   PaPart part[2];
   int qt[2], wk[2];
-  long long blocks[2];
+  bool ok;
 };
+
+constexpr int PA_SLOTS = 512;         // blocks that run at a time: two a CU
 
 inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
   PaPlan r{};
-  const int nseq = a->B / a->G, rep = a->Hq / a->Hkv;
+  r.ok = true;
+  const int nseq = a->B / a->G, rep = a->Hq / a->Hkv, esz = a->dtype == PP_F16 ? 2 : 4;
   const long long R = (long long)a->Lq * rep;
-  const bool packed = a->P > 0 && nseq > 1 && R <= 32;
-  auto add = [&](int nper, int prefix, int suffix) {
-    PaPart& t = r.part[r.nparts];
-    t.nper = nper; t.prefix = prefix; t.suffix = suffix;
+  // rows of several sequences are packed where one sequence's do not fill a tile and re-reading the prefix for each would move 16 MB or more
+  const bool packed = a->P > 0 && nseq > 1 && R <= 32 && (long long)(a->B - a->G) * a->Hkv * a->P * a->D * 2 * esz >= (16 << 20);
+  auto add = [&](int nper, int prefix, int suffix, int most, bool both) {
+    const int i = r.nparts++;
+    PaPart& t = r.part[i];
+    t.nper = nper; t.prefix = prefix; t.suffix = suffix; t.by_row = both;
     t.rows = (int)(R * nper);
-    int& qt = r.qt[r.nparts];
-    int& wk = r.wk[r.nparts];
-    wk = t.rows <= 32;
-    qt = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 ? 1 : 2;
-    const int per = 16 * qt * (wk ? 1 : 4);
+    r.wk[i] = t.rows <= 32;
+    r.qt[i] = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 ? 1 : 2;
+    const int per = 16 * r.qt[i] * (r.wk[i] ? 1 : 4);
     t.rowblocks = ceil_div(t.rows, per);
-    const long long blocks = (long long)(a->B / nper) * a->Hkv * t.rowblocks;
-    const int kt = a->dtype == PP_F16 && wk ? 128 : 64;
+    const long long items = (long long)(a->B / nper) * a->Hkv * t.rowblocks;
+    if (items > (1 << 22)) { r.ok = false; return; }
+    t.items = (int)items;
+    const int kt = a->dtype == PP_F16 && r.wk[i] ? 128 : 64;
     const int tiles = (prefix ? ceil_div(a->P, kt) : 0) + (suffix ? ceil_div(a->S, kt) : 0);
-    long long n = blocks > 0 ? 512 / blocks : 1;
-    if (n > tiles / 2) n = tiles / 2;
+    // items that fill whole rounds walk their keys alone; those of the last, incomplete round are split until it is full too, four tiles a block at least
+    const int rest = both ? t.items : t.items % PA_SLOTS;
+    int n = rest > 0 ? most / rest : 1;
+    if (n > tiles / 4) n = tiles / 4;
     if (n > 32) n = 32;
     if (n < 1) n = 1;
-    t.nsplit = (int)n;
+    t.nsplit = n;
+    t.whole = both ? 0 : n == 1 ? t.items : t.items - rest;
     t.slot0 = r.slots;
-    r.slots += t.nsplit;
-    r.blocks[r.nparts] = blocks * n;
-    ++r.nparts;
+    t.blocks = t.whole + (t.items - t.whole) * n;
+    if (both) r.prows = (long long)a->B * a->Lq * a->Hq;
+    else r.prows = (long long)(t.items - t.whole) * per;
+    if (t.whole < t.items) r.slots += n;
   };
-  if (packed) {
-    add(nseq, 1, 0);
-    if (a->S > 0) add(1, 0, 1);
+  if (packed && a->S > 0) {
+    add(1, 0, 1, PA_SLOTS, true);
+    add(nseq, 1, 0, PA_SLOTS / 2, true);
+  } else if (packed) {
+    add(nseq, 1, 0, PA_SLOTS, false);
   } else {
-    add(1, a->P > 0, a->S > 0);
+    add(1, a->P > 0, a->S > 0, PA_SLOTS, false);
   }
   return r;
 }
+inline int64_t pa_scratch(const PaPlan& plan, int D) { return plan.slots * plan.prows * (D + 2) * 4; }
 
 template <typename T, int D>
-static void pa_launch(const PaPlan& plan, PaParams p, hipStream_t st) {
-  for (int i = 0; i < plan.nparts; ++i) {
-    p.part = plan.part[i];
-    const dim3 grid((unsigned)plan.blocks[i]), block(256);
-    if (plan.wk[i]) {
-      if (plan.qt[i] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, true>), grid, block, 0, st, p);
+static void pa_launch(const PaPlan& plan, const PaParams& p, hipStream_t st) {
+  const dim3 block(256);
+  if (plan.nparts == 2) {
+    const dim3 grid((unsigned)(plan.part[0].blocks + plan.part[1].blocks));
+    const int form = plan.wk[1] ? plan.qt[1] - 1 : 1 + plan.qt[1];      // of the packed part: wk 1, wk 2, rows 1, rows 2; the suffix part is always wk
+#define PA_PAIR(Q0, Q1, W1) hipLaunchKernelGGL((pa_pair_kernel<T, D, Q0, true, Q1, W1>), grid, block, 0, st, p)
+    if (plan.qt[0] == 1) {
+      if (form == 0) PA_PAIR(1, 1, true);
+      else if (form == 1) PA_PAIR(1, 2, true);
+      else if (form == 2) PA_PAIR(1, 1, false);
+      else PA_PAIR(1, 2, false);
+    } else {
+      if (form == 2) PA_PAIR(2, 1, false);
+      else PA_PAIR(2, 2, false);
+    }
+#undef PA_PAIR
+  } else {
+    const dim3 grid((unsigned)plan.part[0].blocks);
+    if (plan.wk[0]) {
+      if (plan.qt[0] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, true>), grid, block, 0, st, p);
       else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, true>), grid, block, 0, st, p);
     } else {
-      if (plan.qt[i] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, false>), grid, block, 0, st, p);
+      if (plan.qt[0] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, false>), grid, block, 0, st, p);
       else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, false>), grid, block, 0, st, p);
     }
   }
-  if (plan.slots > 1)
-    hipLaunchKernelGGL((pa_join_kernel<T, D>), dim3((unsigned)(((long long)p.B * p.Lq * p.Hq + 3) / 4)), dim3(256), 0, st, p);
+  if (plan.slots > 0)
+    hipLaunchKernelGGL((pa_join_kernel<T, D>), dim3((unsigned)((plan.prows + 3) / 4)), block, 0, st, p, 16 * plan.qt[0] * (plan.wk[0] ? 1 : 4));
 }
 
 }  // namespace pp
@@ -494,7 +583,8 @@ extern "C" int64_t pp_shared_prefix_attention_workspace_bytes(const pp_prefix_at
   if (rc != 0) return rc;
   if (a->B == 0 || a->Lq == 0) return 0;
   const PaPlan plan = pa_plan(a);
-  return plan.slots > 1 ? (int64_t)plan.slots * a->B * a->Lq * a->Hq * (a->D + 2) * 4 : 0;
+  PP_REQUIRE(plan.ok, PP_ERR_ARG, "pp_shared_prefix_attention: too many blocks of work");
+  return pa_scratch(plan, a->D);
 }
 
 static int pa_check_tensor(const char* name, const void* ptr, const int64_t* st, int n0, int n1, int n2, int D, int dtype) {
@@ -529,6 +619,7 @@ extern "C" int pp_shared_prefix_attention(const pp_prefix_attn_args_t* a, void* 
     if ((rc = pa_check_tensor("v", a->v, a->v_stride, a->B, a->S, a->Hkv, a->D, a->dtype)) != 0) return rc;
   }
   const int64_t need = pp_shared_prefix_attention_workspace_bytes(a);
+  if (need < 0) return (int)need;
   PP_REQUIRE(need == 0 || (a->work != nullptr && a->work_bytes >= need && (uintptr_t)a->work % 16 == 0), PP_ERR_WORKSPACE,
              "pp_shared_prefix_attention: needs %lld bytes of 16-byte aligned scratch, got %lld", (long long)need, (long long)a->work_bytes);
   PaParams p;
@@ -543,10 +634,12 @@ extern "C" int pp_shared_prefix_attention(const pp_prefix_attn_args_t* a, void* 
   p.sc2 = a->scale != 0.f ? fabsf(a->scale) * 1.4426950408889634f : 1.f;
   p.qsign = a->scale > 0.f ? 1.f : a->scale < 0.f ? -1.f : 0.f;
   const PaPlan plan = pa_plan(a);
-  PP_REQUIRE(plan.blocks[0] <= (1 << 23) && plan.blocks[1] <= (1 << 23), PP_ERR_ARG, "pp_shared_prefix_attention: too many blocks of work");
   p.slots = plan.slots;
-  p.part_o = plan.slots > 1 ? (float*)a->work : nullptr;
-  p.part_ml = plan.slots > 1 ? (float*)a->work + (int64_t)plan.slots * a->B * a->Lq * a->Hq * a->D : nullptr;
+  p.prows = plan.prows;
+  p.part[0] = plan.part[0];
+  p.part[1] = plan.part[1];
+  p.part_o = (float*)a->work;
+  p.part_ml = (float*)a->work + plan.slots * plan.prows * a->D;
   hipStream_t st = (hipStream_t)stream;
   if (a->dtype == PP_F16) {
     if (a->D == 128) pa_launch<_Float16, 128>(plan, p, st);
