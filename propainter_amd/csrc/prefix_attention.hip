@@ -83,16 +83,26 @@ template <typename T, int D, bool WK> struct PaTile {
   static constexpr int NK = WK ? KT / 64 : 4;                 // 16-key tiles of a wave
   static constexpr int SLOTS = D * (int)sizeof(T) / 16;       // 16-byte slots of a key row
   static constexpr int STEPS = SLOTS / 4;                     // fragments of a row
-  static constexpr int VLD = F16 ? D + 4 : D + 16;            // V row stride (elements): skews the banks of a column's keys
+  static constexpr int VLD = F16 ? D : D + 16;                // V row stride (elements); fp16 rows are swizzled (v_at), fp32 rows skewed
   static constexpr int LOADS = KT * SLOTS / 256;              // 16-byte pieces a thread stages of K and of V
   static constexpr int KBYTES = KT * D * (int)sizeof(T), VBYTES = KT * VLD * (int)sizeof(T);
 };
+
+// fp16 V rows: 16-byte slot s (8 channels) of key k lies in slot s ^ f(k), its 8-byte halves swapped where k & 4 -- the 8 keys x 4 halves that 32
+// lanes of a transposing read take then cover all 64 banks once.
+template <int D> __device__ __forceinline__ int v_slot(int key, int s) { return s ^ (D == 128 ? (key & 3) << 2 : (key & 2) << 1); }
 
 template <typename T, int D, int QT, bool WK> struct PaLds {
   typedef PaTile<T, D, WK> C;
   static constexpr int JOIN = WK ? 4 * 16 * QT * (D + 4) * 4 : 0;
   static constexpr int BYTES = C::KBYTES + C::VBYTES > JOIN ? C::KBYTES + C::VBYTES : JOIN;
 };
+
+// channel of position `pos` (of 4 neighbours) of an accumulator row: see the product with V
+template <bool F16> __device__ __forceinline__ int pa_channel(int pos) {
+  const int d = pos >> 4, g = (pos >> 2) & 3;
+  return F16 ? (d >> 1) * 32 + g * 8 + (d & 1) * 4 + (pos & 3) : pos;
+}
 
 // block `bid` of part `pt`
 template <typename T, int D, int QT, bool WK>
@@ -204,14 +214,11 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     for (int i = 0; i < C::LOADS; ++i) {
       const int c = tid + 256 * i, key = c / C::SLOTS, sl = c % C::SLOTS;
       *reinterpret_cast<u32x4*>(&Ks[key * D + (sl ^ swz(key)) * (16 / sizeof(T))]) = kr[i];
-      T* vrow = &Vs[key * C::VLD + sl * (16 / sizeof(T))];
-      if constexpr (C::F16) {                      // rows are 8-byte aligned: two halves, in opposite order in the two halves of a row
-        const int sel = sl >= C::SLOTS / 2;
-        const u32x2 lo = {vr[i][0], vr[i][1]}, hi = {vr[i][2], vr[i][3]};
-        *reinterpret_cast<u32x2*>(vrow + sel * 4) = sel ? hi : lo;
-        *reinterpret_cast<u32x2*>(vrow + (sel ^ 1) * 4) = sel ? lo : hi;
+      if constexpr (C::F16) {
+        const u32x4 v = key & 4 ? u32x4{vr[i][2], vr[i][3], vr[i][0], vr[i][1]} : vr[i];
+        *reinterpret_cast<u32x4*>(&Vs[key * C::VLD + v_slot<D>(key, sl) * 8]) = v;
       } else {
-        *reinterpret_cast<u32x4*>(vrow) = vr[i];
+        *reinterpret_cast<u32x4*>(&Vs[key * C::VLD + sl * 4]) = vr[i];
       }
     }
   };
@@ -281,14 +288,16 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     // ---- O^T += V^T P^T
     if constexpr (C::F16) {
       // contraction slot lg * 8 + e of a 32-key step is key (e >> 2) * 16 + lg * 4 + (e & 3); accumulator row i of tile d is channel
-      // (i / 4) * (D / 4) + d * 4 + i % 4: a lane ends with D / 4 consecutive channels of its query
-      const _Float16* vb = reinterpret_cast<const _Float16*>(Vs) + (wkey + lg * 4 + (lc >> 2)) * C::VLD + (lane & 3) * (D / 4);
+      // (d / 2) * 32 + (i / 4) * 8 + (d % 2) * 4 + i % 4: two tiles give a lane 8 consecutive channels, four lanes 64 bytes of a row
+      const int key = wkey + lg * 4 + (lc >> 2);          // (+ 16, + 32: the swizzle looks at its low bits only)
+      const _Float16* vb = reinterpret_cast<const _Float16*>(Vs) + key * C::VLD;
 #pragma unroll
       for (int j = 0; j < NK / 2; ++j)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const f16x4 v0 = lds_read_tr16(vb + 32 * j * C::VLD + d * 4);
-          const f16x4 v1 = lds_read_tr16(vb + (32 * j + 16) * C::VLD + d * 4);
+          const int at = v_slot<D>(key, (d >> 1) * 4 + (lane & 3)) * 8 + (((d & 1) ^ ((key >> 2) & 1)) << 2);
+          const f16x4 v0 = lds_read_tr16(vb + 32 * j * C::VLD + at);
+          const f16x4 v1 = lds_read_tr16(vb + (32 * j + 16) * C::VLD + at);
           const f16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pfr[qt][j], oacc[qt][d], 0, 0, 0);
@@ -310,8 +319,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     __syncthreads();
   }
 
-  // channel of accumulator element (d, r) of this lane
-  auto chan = [&](int d, int r) { return C::F16 ? lg * (D / 4) + d * 4 + r : d * 16 + lg * 4 + r; };
+  // Accumulator element (d, r) of lane group lg is position d * 16 + lg * 4 + r of its row; scratch rows are kept in that order.
   if constexpr (!WK) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -322,7 +330,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
         if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_run[qt], l);
         if (t0 < t1) {
 #pragma unroll
-          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + chan(d, 0)) = oacc[qt][d];
+          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + d * 16 + lg * 4) = oacc[qt][d];
         }
       } else {
         const float inv = l != 0.f ? 1.f / l : 0.f;           // no keys: zeros
@@ -333,11 +341,11 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
             float v[8];
 #pragma unroll
             for (int r = 0; r < 4; ++r) { v[r] = oacc[qt][d][r] * inv; v[4 + r] = oacc[qt][d + 1][r] * inv; }
-            store8<T>(o + chan(d, 0), v);
+            store8<T>(o + pa_channel<C::F16>(d * 16 + lg * 4), v);
           }
         } else {
 #pragma unroll
-          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + chan(d, 0)) = oacc[qt][d] * inv;
+          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + d * 16 + lg * 4) = oacc[qt][d] * inv;
         }
       }
     }
@@ -366,31 +374,31 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
       for (int w = 0; w < 4; ++w) lj[qt] += e[w * W + 1] * __builtin_amdgcn_exp2f(e[w * W] - mj[qt]);
       const float f = __builtin_amdgcn_exp2f(m_run[qt] - mj[qt]);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + chan(d, 0)) = oacc[qt][d] * f;
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + d * 16 + lg * 4) = oacc[qt][d] * f;
     }
     __syncthreads();
-    // wave w finishes rows lc of its quarter of the channels: lane -> row lc, channels wave * D / 4 + lg * D / 16 ..
+    // wave w finishes positions w * D / 4 .. of rows lc: 16 rows x 4 lane groups x D / 64 pieces of 4
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       if (rowid[qt] < 0) continue;
-      const int c0 = wave * (D / 4) + lg * (D / 16);
-      const float* e = jo + (qt * 16 + lc) * JLD + c0;
+      const float* e = jo + (qt * 16 + lc) * JLD;
       constexpr int W = 16 * QT * JLD;
       const float inv = lj[qt] != 0.f ? 1.f / lj[qt] : 0.f;
       const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
       if (!whole && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
 #pragma unroll
-      for (int c = 0; c < D / 16; c += 4) {
-        f32x4 v = *reinterpret_cast<const f32x4*>(e + c);
+      for (int c = 0; c < D / 64; ++c) {
+        const int pos = wave * (D / 4) + c * 16 + lg * 4;
+        f32x4 v = *reinterpret_cast<const f32x4*>(e + pos);
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + c);
+        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + pos);
         if (!whole) {
-          if (t0 < t1) *reinterpret_cast<f32x4*>(p.part_o + at * D + c0 + c) = v;
+          if (t0 < t1) *reinterpret_cast<f32x4*>(p.part_o + at * D + pos) = v;
         } else if constexpr (C::F16) {
           const f16x4 o = {(_Float16)(v[0] * inv), (_Float16)(v[1] * inv), (_Float16)(v[2] * inv), (_Float16)(v[3] * inv)};
-          *reinterpret_cast<f16x4*>(reinterpret_cast<T*>(optr[qt]) + c0 + c) = o;
+          *reinterpret_cast<f16x4*>(reinterpret_cast<T*>(optr[qt]) + pa_channel<C::F16>(pos)) = o;
         } else {
-          *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(optr[qt]) + c0 + c) = v * inv;
+          *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(optr[qt]) + pos) = v * inv;
         }
       }
     }
@@ -398,8 +406,6 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
 #endif
 }
 
-// One part a launch, or the two parts of a call in one, the packed rows' products (part 1) first: they run next to the memory-bound walks of the
-// suffixes (part 0).
 // waves a SIMD the registers are to allow: two blocks a CU, but for fp32 heads of 128 in two row tiles, which do not fit
 template <typename T, int D, int QT> constexpr int pa_waves() { return sizeof(T) == 4 && D == 128 && QT == 2 ? 1 : 2; }
 
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p, const in
       for (int e = 0; e < E; ++e) acc[e] = s0 + u < p.slots && ls != 0.f ? fmaf(ws, v[u][e], acc[e]) : acc[e];
     }
   }
-  T* o = reinterpret_cast<T*>(p.out) + w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2] + lane * E;
+  T* o = reinterpret_cast<T*>(p.out) + w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2] + pa_channel<sizeof(T) == 2>(lane * E);
   const float inv = total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
@@ -507,7 +513,9 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
     // items that fill whole rounds walk their keys alone; those of the last, incomplete round are split until it is full too, four tiles a block at least
     const int rest = both ? t.items : t.items % PA_SLOTS;
     int n = rest > 0 ? most / rest : 1;
-    if (n > tiles / 4) n = tiles / 4;
+    const int least = r.wk[i] ? 1 : a->dtype == PP_F16 ? 4 : 2;
+    if (n > tiles / least) n = tiles / least;
+    if (!both && tiles < 4) n = 1;
     if (n > 32) n = 32;
     if (n < 1) n = 1;
     t.nsplit = n;
