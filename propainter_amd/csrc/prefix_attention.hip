@@ -104,6 +104,91 @@ template <bool F16> __device__ __forceinline__ int pa_channel(int pos) {
   return F16 ? (d >> 1) * 32 + g * 8 + (d & 1) * 4 + (pos & 3) : pos;
 }
 
+// block -> item (row block fastest, key head, row space) and key split
+struct PaItem { bool whole; int item, split, rb, hk, space; };
+__device__ __forceinline__ PaItem pa_item(const PaParams& p, const PaPart& pt, const int bid) {
+  int item, split = 0;
+  const bool whole = bid < pt.whole;
+  if (whole) {
+    item = xcd_run(bid, pt.whole);
+  } else {
+    const int x = xcd_run(bid - pt.whole, pt.blocks - pt.whole), rest = pt.items - pt.whole;
+    if (pt.whole == 0) {      // row blocks of one space and split are neighbours
+      const int rb = x % pt.rowblocks, y = x / pt.rowblocks;
+      split = y % pt.nsplit;
+      item = y / pt.nsplit * pt.rowblocks + rb;
+    } else {
+      split = x / rest;
+      item = pt.whole + x % rest;
+    }
+  }
+  return {whole, item, split, item % pt.rowblocks, item / pt.rowblocks % p.Hkv, item / pt.rowblocks / p.Hkv};
+}
+
+// The four waves of a block hold the same 16 QT rows for different keys: joined through LDS, then written out (or left in the scratch)
+template <typename T, int D, int QT>
+__device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& pt, char* lds, float* wave_ml, const f32x4 (&oacc)[QT][D / 16], const float (&m_run)[QT],
+                                              const float (&l_run)[QT], const long long (&rowid)[QT], char* const (&optr)[QT], const bool whole, const int split,
+                                              const bool any) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr bool F16 = sizeof(T) == 2;
+  constexpr int DT = D / 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lg = lane >> 4, lc = lane & 15;
+  // every wave scales its rows to the common maximum, LDS holds [wave][row][D + 4] floats
+  float* jo = reinterpret_cast<float*>(lds);
+  constexpr int JLD = D + 4;
+  float l[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    l[qt] = rows_sum(l_run[qt]);
+    if (lg == 0) {
+      wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2] = m_run[qt];
+      wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2 + 1] = l[qt];
+    }
+  }
+  __syncthreads();
+  float mj[QT], lj[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float* e = wave_ml + (qt * 16 + lc) * 2;
+    constexpr int W = 16 * QT * 2;
+    mj[qt] = fmaxf(fmaxf(e[0], e[W]), fmaxf(e[2 * W], e[3 * W]));
+    lj[qt] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) lj[qt] += e[w * W + 1] * __builtin_amdgcn_exp2f(e[w * W] - mj[qt]);
+    const float f = __builtin_amdgcn_exp2f(m_run[qt] - mj[qt]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + d * 16 + lg * 4) = oacc[qt][d] * f;
+  }
+  __syncthreads();
+  // wave w finishes positions w * D / 4 .. of rows lc: 16 rows x 4 lane groups x D / 64 pieces of 4
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    if (rowid[qt] < 0) continue;
+    const float* e = jo + (qt * 16 + lc) * JLD;
+    constexpr int W = 16 * QT * JLD;
+    const float inv = lj[qt] != 0.f ? 1.f / lj[qt] : 0.f;
+    const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
+    if (!whole && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      const int pos = wave * (D / 4) + c * 16 + lg * 4;
+      f32x4 v = *reinterpret_cast<const f32x4*>(e + pos);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + pos);
+      if (!whole) {
+        if (any) *reinterpret_cast<f32x4*>(p.part_o + at * D + pos) = v;
+      } else if constexpr (F16) {
+        const f16x4 o = {(_Float16)(v[0] * inv), (_Float16)(v[1] * inv), (_Float16)(v[2] * inv), (_Float16)(v[3] * inv)};
+        *reinterpret_cast<f16x4*>(reinterpret_cast<T*>(optr[qt]) + pa_channel<F16>(pos)) = o;
+      } else {
+        *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(optr[qt]) + pos) = v * inv;
+      }
+    }
+  }
+#endif
+}
+
 // block `bid` of part `pt`
 template <typename T, int D, int QT, bool WK>
 __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, const int bid, char* lds, float* wave_ml) {
@@ -114,27 +199,9 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
   T* Ks = reinterpret_cast<T*>(lds);
   T* Vs = reinterpret_cast<T*>(lds + C::KBYTES);
 
-  // ---- block -> item (row block fastest, key head, row space) and key split
-  int item, split = 0;
-  const bool whole = bid < pt.whole;
-  if (whole) {
-    item = xcd_run(bid, pt.whole);
-  } else {
-    const int x = xcd_run(bid - pt.whole, pt.blocks - pt.whole), rest = pt.items - pt.whole;
-    // row blocks of one space and split are neighbours where they all are split
-    if (pt.whole == 0) {
-      const int rb = x % pt.rowblocks, y = x / pt.rowblocks;
-      split = y % pt.nsplit;
-      item = y / pt.nsplit * pt.rowblocks + rb;
-    } else {
-      split = x / rest;
-      item = pt.whole + x % rest;
-    }
-  }
-  const int nsplit = whole ? 1 : pt.nsplit;
-  const int rb = item % pt.rowblocks;
-  const int hk = item / pt.rowblocks % p.Hkv;
-  const int space = item / pt.rowblocks / p.Hkv;
+  const PaItem it = pa_item(p, pt, bid);
+  const bool whole = it.whole;
+  const int item = it.item, split = it.split, nsplit = whole ? 1 : pt.nsplit, rb = it.rb, hk = it.hk, space = it.space;
   const int b0 = space * pt.nper, g = b0 / p.nseq;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lg = lane >> 4, lc = lane & 15;
   const int row0 = rb * 16 * QT * (WK ? 1 : 4);
@@ -185,8 +252,8 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- staging: a tile's valid keys lie inside the buffer descriptor built for it, the rest comes back as zeros (so that nothing behind a
-  // length is used); 64-bit base per tile, 32-bit offsets inside it
+  // ---- staging: a tile's valid keys lie inside the buffer descriptor built for it, the rest (token strides are at least D) comes back as zeros,
+  // so that nothing behind a length is used; 64-bit base per tile, 32-bit offsets inside it
   u32x4 kr[C::LOADS], vr[C::LOADS];
   auto tile_keys = [&](int t) {                    // valid keys of tile t
     return t < ptiles ? min(KT, np - t * KT) : min(KT, vis_max - (t - ptiles) * KT);
@@ -204,8 +271,8 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
 #pragma unroll
     for (int i = 0; i < C::LOADS; ++i) {
       const int c = tid + 256 * i, key = c / C::SLOTS, sl = c % C::SLOTS;
-      kr[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(key < n ? key * kp + sl * 16 : 0xfffffff0u), 0, 0);
-      vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(key < n ? key * vp + sl * 16 : 0xfffffff0u), 0, 0);
+      kr[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(key * kp + sl * 16), 0, 0);
+      vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(key * vp + sl * 16), 0, 0);
     }
   };
   auto swz = [](int key) { return C::SLOTS >= 16 ? key & 15 : (key >> 1) & 7; };
@@ -350,60 +417,194 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
       }
     }
   } else {
-    // join the four waves: every wave scales its rows to the common maximum, LDS holds [wave][row][D + 4] floats
-    float* jo = reinterpret_cast<float*>(lds);
-    constexpr int JLD = D + 4;
-    float l[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      l[qt] = rows_sum(l_run[qt]);
-      if (lg == 0) {
-        wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2] = m_run[qt];
-        wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2 + 1] = l[qt];
-      }
-    }
-    __syncthreads();
-    float mj[QT], lj[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const float* e = wave_ml + (qt * 16 + lc) * 2;
-      constexpr int W = 16 * QT * 2;
-      mj[qt] = fmaxf(fmaxf(e[0], e[W]), fmaxf(e[2 * W], e[3 * W]));
-      lj[qt] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) lj[qt] += e[w * W + 1] * __builtin_amdgcn_exp2f(e[w * W] - mj[qt]);
-      const float f = __builtin_amdgcn_exp2f(m_run[qt] - mj[qt]);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + d * 16 + lg * 4) = oacc[qt][d] * f;
-    }
-    __syncthreads();
-    // wave w finishes positions w * D / 4 .. of rows lc: 16 rows x 4 lane groups x D / 64 pieces of 4
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      if (rowid[qt] < 0) continue;
-      const float* e = jo + (qt * 16 + lc) * JLD;
-      constexpr int W = 16 * QT * JLD;
-      const float inv = lj[qt] != 0.f ? 1.f / lj[qt] : 0.f;
-      const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
-      if (!whole && wave == 0 && lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj[qt], lj[qt]);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const int pos = wave * (D / 4) + c * 16 + lg * 4;
-        f32x4 v = *reinterpret_cast<const f32x4*>(e + pos);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + pos);
-        if (!whole) {
-          if (t0 < t1) *reinterpret_cast<f32x4*>(p.part_o + at * D + pos) = v;
-        } else if constexpr (C::F16) {
-          const f16x4 o = {(_Float16)(v[0] * inv), (_Float16)(v[1] * inv), (_Float16)(v[2] * inv), (_Float16)(v[3] * inv)};
-          *reinterpret_cast<f16x4*>(reinterpret_cast<T*>(optr[qt]) + pa_channel<C::F16>(pos)) = o;
-        } else {
-          *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(optr[qt]) + pos) = v * inv;
-        }
-      }
-    }
+    pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, m_run, l_run, rowid, optr, whole, split, t0 < t1);
   }
 #endif
+}
+
+// fp16, few rows: every wave streams 32-key chunks of its own (chunk t0 + wave, then every fourth), with no barrier until the end.  K goes from
+// memory into the operand registers as it is (a chunk's keys are read by one wave only), V through 8 KB of the wave's own LDS for the
+// transposing read; the loads of the next DEPTH chunks are in flight during a chunk's products.
+template <int D, int QT> struct PaStream {
+  static constexpr int DEPTH = QT == 1 ? 2 : 1;
+  static constexpr int VBYTES = 32 * D * 2;
+  static constexpr int JOIN = 4 * 16 * QT * (D + 4) * 4;
+  static constexpr int BYTES = 4 * VBYTES > JOIN ? 4 * VBYTES : JOIN;
+};
+template <int D, int QT>
+__device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart& pt, const int bid, char* lds, float* wave_ml) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef _Float16 T;
+  typedef PaStream<D, QT> C;
+  constexpr int STEPS = D / 32, DT = D / 16, SLOTS = D / 8, VL = 32 * SLOTS / 64, KT = 32;     // VL: V loads a lane and chunk
+  const PaItem it = pa_item(p, pt, bid);
+  const bool whole = it.whole;
+  const int nsplit = whole ? 1 : pt.nsplit, b0 = it.space * pt.nper, g = b0 / p.nseq, hk = it.hk;
+  const int lane = threadIdx.x & 63, lg = lane >> 4, lc = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // provably uniform: chunks, descriptors and branches stay scalar
+  const int row0 = it.rb * 16 * QT, row_end = min(pt.rows, row0 + 16 * QT);
+  T* Vs = reinterpret_cast<T*>(lds + wave * C::VBYTES);
+
+  const int np = pt.prefix ? clamp_len(p.plens, g, p.P) : 0;
+  const int ns = pt.suffix ? clamp_len(p.lens, b0, p.S) : 0;
+  int vis_min = ns, vis_max = ns;                 // suffix keys the block's first / last row sees
+  if (pt.suffix && p.causal) {
+    vis_min = min(ns, max(0, ns - p.Lq + row0 / p.rep + 1));
+    vis_max = min(ns, max(0, ns - p.Lq + (row_end - 1) / p.rep + 1));
+  }
+  const int ptiles = (np + KT - 1) / KT, tiles = ptiles + (vis_max + KT - 1) / KT;
+  const int t0 = (int)((long long)tiles * it.split / nsplit), t1 = (int)((long long)tiles * (it.split + 1) / nsplit);
+
+  f16x8 qf[QT][STEPS];
+  long long rowid[QT];
+  int vis[QT];
+  char* optr[QT];
+  f32x4 oacc[QT][DT];
+  float m_run[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rl = qt * 16 + lc, r = row0 + rl;
+    const bool ok = r < pt.rows;
+    const PaRow w = pa_row(p.Lq, p.rep, pt.nper, it.space, hk, ok ? r : 0);
+    rowid[qt] = !ok ? -1 : whole ? 0 : pt.by_row ? ((long long)w.b * p.Lq + w.i) * p.Hq + w.h : (long long)(it.item - pt.whole) * (16 * QT) + rl;
+    vis[qt] = p.causal ? max(0, ns - p.Lq + w.i + 1) : ns;
+    optr[qt] = p.out + (w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2]) * 2;
+    const T* qp = reinterpret_cast<const T*>(p.q) + w.b * p.qs[0] + w.i * p.qs[1] + w.h * p.qs[2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      f16x8 f = *reinterpret_cast<const f16x8*>(qp + (s * 4 + lg) * 8);
+      if (p.qsign != 1.f) f *= (T)p.qsign;
+      qf[qt][s] = f;
+    }
+    m_run[qt] = PA_NONE;
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  u32x4 kf[C::DEPTH][2][STEPS], vr[C::DEPTH][VL];
+  auto keys_of = [&](int t) { return t >= t1 ? 0 : t < ptiles ? min(KT, np - t * KT) : min(KT, vis_max - (t - ptiles) * KT); };
+  // (issued for every chunk, those past the last one with an empty descriptor: with a load that may or may not be there the wait for an older
+  // one would be a wait for all)
+  auto load = [&](int t, int set) {
+    const bool pre = t < ptiles;
+    const long long j0 = t < t1 ? (long long)(pre ? t : t - ptiles) * KT : 0;
+    const long long kts = pre ? p.pks[1] : p.ks[1], vts = pre ? p.pvs[1] : p.vs[1];
+    const T* kb = pre ? reinterpret_cast<const T*>(p.pk) + g * p.pks[0] + hk * p.pks[2] : reinterpret_cast<const T*>(p.k) + b0 * p.ks[0] + hk * p.ks[2];
+    const T* vb = pre ? reinterpret_cast<const T*>(p.pv) + g * p.pvs[0] + hk * p.pvs[2] : reinterpret_cast<const T*>(p.v) + b0 * p.vs[0] + hk * p.vs[2];
+    const unsigned kp = (unsigned)kts * 2, vp = (unsigned)vts * 2;
+    const int n = keys_of(t);
+    const __amdgpu_buffer_rsrc_t rk = uniform_buffer_rsrc(kb + j0 * kts, n > 0 ? (int)((n - 1) * kp + D * 2) : 0);
+    const __amdgpu_buffer_rsrc_t rv = uniform_buffer_rsrc(vb + j0 * vts, n > 0 ? (int)((n - 1) * vp + D * 2) : 0);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int key = kt * 16 + lc;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        kf[set][kt][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(key * kp + (s * 4 + lg) * 16), 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = (i * 64 + lane) / SLOTS, sl = lane % SLOTS;
+      vr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(key * vp + sl * 16), 0, 0);
+    }
+  };
+  auto chunk = [&](int t, int set) {
+    // V of the chunk: rows into the wave's own LDS (its earlier reads are ahead of these writes in the LDS queue)
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = (i * 64 + lane) / SLOTS, sl = lane % SLOTS;
+      const u32x4 v = key & 4 ? u32x4{vr[set][i][2], vr[set][i][3], vr[set][i][0], vr[set][i][1]} : vr[set][i];
+      *reinterpret_cast<u32x4*>(&Vs[key * D + v_slot<D>(key, sl) * 8]) = v;
+    }
+    // its operands, all requested here: they arrive during the scores and the softmax (read one by one ahead of each product they made up most
+    // of a chunk's time)
+    f16x8 vf[DT];
+    {
+      const int key = lg * 4 + (lc >> 2);
+      const _Float16* vb = Vs + key * D;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int at = v_slot<D>(key, (d >> 1) * 4 + (lane & 3)) * 8 + (((d & 1) ^ ((key >> 2) & 1)) << 2);
+        const f16x4 v0 = lds_read_tr16(vb + at);
+        const f16x4 v1 = lds_read_tr16(vb + 16 * D + at);
+        vf[d] = f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 sacc[QT][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        sacc[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+          sacc[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[set][kt][s]), qf[qt][s], sacc[qt][kt], 0, 0, 0);
+      }
+    const int n = keys_of(t), j0 = (t - ptiles) * KT;
+    const bool cut = p.causal && t >= ptiles && j0 + n > vis_min;
+    f16x8 pfr[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if (n < KT || cut) {
+        const int most = cut ? min(n, vis[qt] - j0) : n;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (kt * 16 + lg * 4 + r >= most) sacc[qt][kt][r] = -INFINITY;
+      }
+      float tmax = sacc[qt][0][0];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
+      tmax = rows_max(tmax);
+      const float m_new = fmaxf(m_run[qt], tmax * p.sc2);
+      const bool moved = m_new > m_run[qt];
+      float psum = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, -m_new));
+          psum += e;
+          pfr[qt][kt * 4 + r] = (_Float16)e;             // weights in the values' type: the product's operand
+        }
+      if (__builtin_amdgcn_ballot_w64(moved) != 0ull) {
+        const float alpha = __builtin_amdgcn_exp2f(m_run[qt] - m_new);
+        l_run[qt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oacc[qt][d] *= alpha;
+      }
+      m_run[qt] = m_new;
+      l_run[qt] += psum;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pfr[qt], oacc[qt][d], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(t + 4 * C::DEPTH, set);
+  };
+#pragma unroll
+  for (int i = 0; i < C::DEPTH; ++i) load(t0 + wave + 4 * i, i);
+  for (int t = t0 + wave; t < t1; t += 4 * C::DEPTH) {
+    chunk(t, 0);
+    if constexpr (C::DEPTH == 2) chunk(t + 4, 1);         // (a chunk past the last one has no keys)
+  }
+  __syncthreads();                                         // every wave is done with its V rows: the join takes their place
+  pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, m_run, l_run, rowid, optr, whole, it.split, t0 < t1);
+#endif
+}
+
+// the form of a part: see PaPlan
+template <typename T, int D, int QT, bool WK> constexpr int pa_lds_bytes() { return WK && sizeof(T) == 2 ? PaStream<D, QT>::BYTES : PaLds<T, D, QT, WK>::BYTES; }
+template <typename T, int D, int QT, bool WK>
+__device__ __forceinline__ void pa_run(const PaParams& p, const PaPart& pt, const int bid, char* lds, float* wave_ml) {
+  if constexpr (WK && sizeof(T) == 2) pa_stream_block<D, QT>(p, pt, bid, lds, wave_ml);
+  else pa_block<T, D, QT, WK>(p, pt, bid, lds, wave_ml);
 }
 
 // waves a SIMD the registers are to allow: two blocks a CU, but for fp32 heads of 128 in two row tiles, which do not fit
@@ -411,17 +612,17 @@ template <typename T, int D, int QT> constexpr int pa_waves() { return sizeof(T)
 
 template <typename T, int D, int QT, bool WK>
 __global__ __launch_bounds__(256, (pa_waves<T, D, QT>())) void pa_tile_kernel(const PaParams p) {
-  __shared__ __attribute__((aligned(16))) char lds[PaLds<T, D, QT, WK>::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds[(pa_lds_bytes<T, D, QT, WK>())];
   __shared__ float wave_ml[WK ? 4 * 16 * QT * 2 : 1];
-  pa_block<T, D, QT, WK>(p, p.part[0], (int)blockIdx.x, lds, wave_ml);
+  pa_run<T, D, QT, WK>(p, p.part[0], (int)blockIdx.x, lds, wave_ml);
 }
 template <typename T, int D, int QT0, bool WK0, int QT1, bool WK1>
 __global__ __launch_bounds__(256, (pa_waves<T, D, (QT0 > QT1 ? QT0 : QT1)>())) void pa_pair_kernel(const PaParams p) {
-  constexpr int B0 = PaLds<T, D, QT0, WK0>::BYTES, B1 = PaLds<T, D, QT1, WK1>::BYTES;
+  constexpr int B0 = pa_lds_bytes<T, D, QT0, WK0>(), B1 = pa_lds_bytes<T, D, QT1, WK1>();
   __shared__ __attribute__((aligned(16))) char lds[B0 > B1 ? B0 : B1];
   __shared__ float wave_ml[4 * 16 * 2 * 2];
-  if ((int)blockIdx.x < p.part[1].blocks) pa_block<T, D, QT1, WK1>(p, p.part[1], (int)blockIdx.x, lds, wave_ml);
-  else pa_block<T, D, QT0, WK0>(p, p.part[0], (int)blockIdx.x - p.part[1].blocks, lds, wave_ml);
+  if ((int)blockIdx.x < p.part[1].blocks) pa_run<T, D, QT1, WK1>(p, p.part[1], (int)blockIdx.x, lds, wave_ml);
+  else pa_run<T, D, QT0, WK0>(p, p.part[0], (int)blockIdx.x - p.part[1].blocks, lds, wave_ml);
 }
 
 // One wave per split row: the slots' outputs, weighted by exp2(max - common max), over the weighted sum.  A slot without keys (sum 0) left no output:
@@ -515,7 +716,7 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
     int n = rest > 0 ? most / rest : 1;
     const int least = r.wk[i] ? 1 : a->dtype == PP_F16 ? 4 : 2;
     if (n > tiles / least) n = tiles / least;
-    if (!both && tiles < 4) n = 1;
+    if (!both && tiles < 8) n = 1;      // (a second launch costs more than what is left to split)
     if (n > 32) n = 32;
     if (n < 1) n = 1;
     t.nsplit = n;
@@ -637,6 +838,9 @@ extern "C" int pp_shared_prefix_attention(const pp_prefix_attn_args_t* a, void* 
   long long* to[6] = {p.qs, p.pks, p.pvs, p.ks, p.vs, p.os};
   for (int t = 0; t < 6; ++t)
     for (int i = 0; i < 3; ++i) to[t][i] = from[t][i];
+  // (the stride of a single token is free: keys past it have to lie outside)
+  if (a->P <= 1) p.pks[1] = p.pvs[1] = a->D;
+  if (a->S <= 1) p.ks[1] = p.vs[1] = a->D;
   p.B = a->B; p.G = a->G; p.nseq = a->B / a->G; p.Lq = a->Lq; p.Hq = a->Hq; p.Hkv = a->Hkv; p.rep = a->Hq / a->Hkv; p.P = a->P; p.S = a->S;
   p.causal = a->causal;
   p.sc2 = a->scale != 0.f ? fabsf(a->scale) * 1.4426950408889634f : 1.f;
