@@ -87,7 +87,7 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
   return v;
 }
 
-// Codes of 8 values of a row whose scale needs no lift: v / s rounded by adding 1.5 * 2^23 (the code is the sum's low byte), the remainders'
+// Codes of 8 values of a row whose scale needs no lift (half = s / 2; a negative half sends the others to code_of): v / s rounded by adding 1.5 * 2^23 (the code is the sum's low byte), the remainders'
 // maximum looked at once -- a remainder of half a step or more (ties, and quotients next to one) takes code_of's comparison.
 __device__ __forceinline__ u32x2 codes8_fast(const float* v, const RowScale& r, float half) {
   constexpr float magic = 12582912.f;
@@ -105,7 +105,18 @@ __device__ __forceinline__ u32x2 codes8_fast(const float* v, const RowScale& r, 
     const unsigned lo = __builtin_amdgcn_perm(b[h * 4 + 1], b[h * 4], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[h * 4 + 3], b[h * 4 + 2], 0x0c0c0400u);
     w[h] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   }
-  return worst >= half ? codes8(v, r) : w;
+  if (worst >= half) {
+    float u[8];                                    // (opaque: the rare path's arithmetic stays in it instead of being done for everybody)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u[i] = v[i];
+#if defined(__HIP_DEVICE_COMPILE__)
+      asm volatile("" : "+v"(u[i]));
+#endif
+    }
+    w = codes8(u, r);
+  }
+  return w;
 }
 
 // abs maximum of 8 raw elements, as bits of the element type (fp16: two at a time)
@@ -114,6 +125,7 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 template <> struct Raw8<_Float16> {
   u32x4 r;
   __device__ __forceinline__ void load(const _Float16* p) { r = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void clear() { r = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ void set(int i, _Float16 v) {
     const unsigned u = __builtin_bit_cast(unsigned short, v);
     r[i >> 1] = (i & 1) ? (r[i >> 1] & 0xffffu) | (u << 16) : (r[i >> 1] & 0xffff0000u) | u;
@@ -134,6 +146,7 @@ template <> struct Raw8<_Float16> {
 template <> struct Raw8<float> {
   u32x4 r[2];
   __device__ __forceinline__ void load(const float* p) { r[0] = *reinterpret_cast<const u32x4*>(p); r[1] = *reinterpret_cast<const u32x4*>(p + 4); }
+  __device__ __forceinline__ void clear() { r[0] = r[1] = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ void set(int i, float v) { r[i >> 2][i & 3] = __float_as_uint(v); }
   __device__ __forceinline__ void values(float* v) const {
 #pragma unroll
@@ -147,70 +160,51 @@ template <> struct Raw8<float> {
   }
 };
 
-__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
-
-// R rows in the registers of WPR waves, VPL vectors of 8 a lane and row: one pass over memory.  4 R / WPR rows a block.
-template <typename T, int VPL, int WPR, int R>
+// A row in the registers of WPR waves, VPL vectors of 8 a lane: one pass over memory, 4 / WPR rows a block.  WIDE: K a multiple of 8, rows 16-byte
+// aligned.  Bound by memory: 110160 x 1960 fp16 115 us (5.6 TB/s, a copy's rate), x 512 33 us (5.2 TB/s); with the rare path's arithmetic left to
+// the compiler's hoisting the latter took 45.
+template <typename T, int VPL, int WPR, bool WIDE>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, long long xrs, int8_t* __restrict__ q, long long qrs,
-                                                    float* __restrict__ scale, long long rows, int K, int Kp, int wide) {
+                                                    float* __restrict__ scale, long long rows, int K, int Kp) {
   __shared__ unsigned wm[4];
   const int wave = threadIdx.x >> 6, t = threadIdx.x % (64 * WPR);
-  constexpr int RB = 4 * R / WPR;
-  for (long long row0 = blockIdx.x * (long long)RB; row0 < rows; row0 += gridDim.x * (long long)RB) {
-    Raw8<T> raw[R][VPL];
+  for (long long row0 = blockIdx.x * (long long)(4 / WPR); row0 < rows; row0 += gridDim.x * (long long)(4 / WPR)) {
+    const long long row = row0 + wave / WPR;
+    const T* xr = x + min(row, rows - 1) * xrs;
+    Raw8<T> raw[VPL];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const long long row = min(row0 + wave / WPR * R + k, rows - 1);
-      const T* xr = x + row * xrs;
+    for (int v = 0; v < VPL; ++v) {
+      const int c = (v * 64 * WPR + t) * 8;
+      if constexpr (WIDE) {
+        raw[v].load(xr + (c < K ? c : 0));
+        if (c >= K) raw[v].clear();
+      } else {
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int c = (v * 64 * WPR + t) * 8;
-        if (wide && c + 8 <= K) {
-          raw[k][v].load(xr + c);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) raw[k][v].set(i, c + i < K ? xr[c + i] : (T)0.f);
-        }
+        for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < K ? xr[c + i] : (T)0.f);
       }
     }
-    unsigned mine = 0;                             // lane k: the maximum of row k, so that one division sequence serves R rows
+    unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      unsigned m = 0;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) m = max(m, raw[k][v].amax());
-      m = wave_umax(m);
-      if (R == 1 || (threadIdx.x & 63) == k) mine = m;
-    }
+    for (int v = 0; v < VPL; ++v) m = max(m, raw[v].amax());
+    m = wave_umax(m);
     if constexpr (WPR == 4) {
-      if ((threadIdx.x & 63) == 0) wm[wave] = mine;
+      if ((threadIdx.x & 63) == 0) wm[wave] = m;
       __syncthreads();
-      mine = max(max(wm[0], wm[1]), max(wm[2], wm[3]));
+      m = max(max(wm[0], wm[1]), max(wm[2], wm[3]));
       __syncthreads();
     }
-    const RowScale all = row_scale(mine);
+    if (row >= rows) continue;                             // (WPR == 4: one row a block, always below)
+    const RowScale r = row_scale(__builtin_amdgcn_readfirstlane(m));
+    if (t == 0) scale[row] = r.scale;
+    const float half = !r.zero && r.lift == 1.f ? 0.5f * r.s : -1.f;
+    int8_t* qr = q + row * qrs;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const long long row = row0 + wave / WPR * R + k;
-      if (row >= rows) break;                              // (WPR == 4: one row a block, always below)
-      RowScale r;
-      r.scale = lane_of(all.scale, k);
-      r.s = lane_of(all.s, k);
-      r.rcp = lane_of(all.rcp, k);
-      r.lift = lane_of(all.lift, k);
-      r.zero = __builtin_amdgcn_readlane((int)all.zero, k) != 0;
-      if (t == 0) scale[row] = r.scale;
-      const bool plain = !r.zero && r.lift == 1.f;
-      const float half = 0.5f * r.s;
-      int8_t* qr = q + row * qrs;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int c = (v * 64 * WPR + t) * 8;
-        if (c >= Kp) break;
-        float f[8];
-        raw[k][v].values(f);
-        *reinterpret_cast<u32x2*>(qr + c) = plain ? codes8_fast(f, r, half) : codes8(f, r);
-      }
+    for (int v = 0; v < VPL; ++v) {
+      const int c = (v * 64 * WPR + t) * 8;
+      if (c >= Kp) break;
+      float f[8];
+      raw[v].values(f);
+      *reinterpret_cast<u32x2*>(qr + c) = codes8_fast(f, r, half);
     }
   }
 }
@@ -449,7 +443,7 @@ __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, 
     const int c = v % per * 4096 + threadIdx.x * 8;
     float f[8];
     raw[v].values(f);
-    if (c < Kp) *reinterpret_cast<u32x2*>(codes + row * ld + c) = !r.zero && r.lift == 1.f ? codes8_fast(f, r, 0.5f * r.s) : codes8(f, r);
+    if (c < Kp) *reinterpret_cast<u32x2*>(codes + row * ld + c) = codes8_fast(f, r, !r.zero && r.lift == 1.f ? 0.5f * r.s : -1.f);
   }
   __syncthreads();
   i32x4 acc[TPB][1];
@@ -576,6 +570,7 @@ template <typename TO, int KT>
 __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params p, const int panels, const int groups, const int tiles) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ __attribute__((aligned(1024))) char lds[2 * 4 * KT * 1024];
+  __shared__ float xs[2][64];                      // scales of the tile's tokens
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int panel = (int)(blockIdx.x >> 3) % panels, grp = (int)(blockIdx.x >> 3) / panels * 8 + (int)(blockIdx.x & 7);
   const int nb = panel * 4 + wave, last = (p.N + 63) / 64 - 1;
@@ -590,7 +585,6 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
   Lane8<TO> ch[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) ch[h].load(p, nb * 64 + h * 32 + (lane >> 4) * 8);
-  float xs[4], xn[4];                              // scales of this tile's and the next tile's tokens: a load between the stores would wait for them
   auto issue = [&](int tile, int buf) {
     long long m = tile * 64ll + wave * 16 + (lane & 15);
     if (m >= p.M) m = p.M - 1;
@@ -598,17 +592,19 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
       if (kt < p.ktiles) __builtin_amdgcn_global_load_lds((i8_gptr)(src + kt * 64), (i8_lptr)(lds + ((buf * 4 + wave) * KT + kt) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) xn[mt] = p.xs[min(tile * 64ll + mt * 16 + (lane & 15), p.M - 1)];
+    if (wave == 0) __builtin_amdgcn_global_load_lds((i8_gptr)(p.xs + min(tile * 64ll + lane, p.M - 1)), (i8_lptr)xs[buf], 4, 0, 0);
   };
+  bool full = false;                               // the tile before left 8 or more stores behind this tile's loads
   int buf = 0;
   if (grp < tiles) issue(grp, 0);
   for (int tile = grp; tile < tiles; tile += groups) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // the tile's loads are older than the stores of the tile before: where those are at least 8 (whole tiles of whole blocks: one each for 4 x 16
+    // tokens and 2 x 8 channels, two in fp32) the stores stay in flight
+    if (full) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                  // tile is there for all waves; the other stage, read one tile ago, is free
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) xs[mt] = xn[mt];
     if (tile + groups < tiles) issue(tile + groups, buf ^ 1);
+    full = p.wide_out && nb * 64 + 64 <= p.N && tile * 64ll + 64 <= p.M;
     const char* st = lds + buf * 4 * KT * 1024 + lane * 16;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -616,17 +612,19 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t] = i32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) xf[kt] = kt < p.ktiles ? *reinterpret_cast<const i32x4*>(st + (mt * KT + kt) * 1024) : i32x4{0, 0, 0, 0};
+      for (int kt = 0; kt < KT; ++kt) xf[kt] = *reinterpret_cast<const i32x4*>(st + (mt * KT + kt) * 1024);      // (past the last k tile: anything, times weights of 0)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[kt][t], xf[kt], acc[t], 0, 0, 0);
       const long long m = tile * 64ll + mt * 16 + (lane & 15);
+      const float xm = xs[buf][mt * 16 + (lane & 15)];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
-        ch[h].value(p, xs[mt], &acc[h * 2], v);
-        if (m < p.M) ch[h].store(p, m, v);
+        ch[h].value(p, xm, &acc[h * 2], v);
+        if (full) store8<TO>(reinterpret_cast<TO*>(p.out) + m * p.ors + ch[h].c, v);
+        else if (m < p.M) ch[h].store(p, m, v);
       }
     }
     buf ^= 1;
@@ -671,9 +669,9 @@ static void launch_product(const LinI8Params& p, hipStream_t st) {
   } else if (p.ktiles >= 96 && t256 >= 512) {
     launch_tiles<TO, 256, 256, 2, 4, 4, 1>(p, st);
   } else if (t256w >= 256) {
-    launch_tiles<TO, 128, 256, 2, 4, 3, 1>(p, st);
+    launch_tiles<TO, 128, 256, 2, 4, 3, 4>(p, st);
   } else {
-    launch_tiles<TO, 128, 128, 4, 2, 4, 1>(p, st);
+    launch_tiles<TO, 128, 128, 4, 2, 4, 4>(p, st);
   }
 }
 
@@ -693,21 +691,18 @@ extern "C" int pp_i8_row_bytes(int K) {
 template <typename T>
 static void launch_quant(const void* x, int64_t xrs, void* q, int64_t qrs, float* scale, int64_t rows, int K, int Kp, int wide, hipStream_t st) {
   const int64_t want = K <= 2048 ? (rows + 3) / 4 : rows;
-  dim3 grid((unsigned)(want < 65536 ? want : 65536)), block(256);
-#define PP_QUANT(V, W, R) hipLaunchKernelGGL((quant_kernel<T, V, W, R>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide)
-  if (K <= 1024 && rows >= 32768) {                // enough rows to fill the chip with several in flight a wave
-    grid.x = (unsigned)((want + 3) / 4 < 65536 ? (want + 3) / 4 : 65536);
-    if (K <= 512) PP_QUANT(1, 1, 4);
-    else PP_QUANT(2, 1, 4);
-  }
-  else if (K <= 512) PP_QUANT(1, 1, 1);
-  else if (K <= 1024) PP_QUANT(2, 1, 1);
-  else if (K <= 2048) PP_QUANT(4, 1, 1);
-  else if (K <= 4096) PP_QUANT(2, 4, 1);
-  else if (K <= 8192) PP_QUANT(4, 4, 1);
-  else if (K <= 16384) PP_QUANT(8, 4, 1);
+  const dim3 grid((unsigned)(want < 65536 ? want : 65536)), block(256);
+#define PP_QUANT_FORM(V, W, F) hipLaunchKernelGGL((quant_kernel<T, V, W, F>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp)
+#define PP_QUANT(V, W) do { if (wide && K % 8 == 0) PP_QUANT_FORM(V, W, true); else PP_QUANT_FORM(V, W, false); } while (0)
+  if (K <= 512) PP_QUANT(1, 1);
+  else if (K <= 1024) PP_QUANT(2, 1);
+  else if (K <= 2048) PP_QUANT(4, 1);
+  else if (K <= 4096) PP_QUANT(2, 4);
+  else if (K <= 8192) PP_QUANT(4, 4);
+  else if (K <= 16384) PP_QUANT(8, 4);
   else hipLaunchKernelGGL((quant_row_kernel<T>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide);
 #undef PP_QUANT
+#undef PP_QUANT_FORM
 }
 
 extern "C" int pp_quantize_tokens(const void* x, int64_t x_rstride, void* q, int64_t q_rstride, float* scale, int64_t rows, int K, int dtype,
