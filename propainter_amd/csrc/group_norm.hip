@@ -5,6 +5,8 @@
 //
 // Statistics are held in fp32 as (count, mean, sum of squared deviations) and joined pairwise (Chan et al. 1979): no difference of large
 // sums of squares, so a map whose mean is far from zero loses nothing.  The order of every sum is fixed by the sizes: no atomics.
+// Bound by memory: the map is read twice (the second time partly from the cache) and written once, 4x360x640x64 fp16 in 75 us = 4.7 TB/s of
+// those three passes.
 #include "common.h"
 #include "attn_lanes.h"
 
@@ -91,7 +93,22 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   }
 }
 
-template <typename T>
+// 8 values past the cache: an output that does not fit next to the input would push out what the second read wants
+template <typename T> __device__ __forceinline__ void stream8(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    u32x4 raw;
+    _Float16* h = reinterpret_cast<_Float16*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
+    __builtin_nontemporal_store(raw, reinterpret_cast<u32x4*>(p));
+  } else {
+    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(p));
+    __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4*>(p + 4));
+  }
+}
+
+// STREAM: a template, as the two stores of a run-time choice would be merged into an ordinary one
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   __shared__ float gm[2048], gr[2048];                 // mean and rstd of every group (groups <= C <= 2048)
   __shared__ float part_n[256], part_m[256], part_v[256];
@@ -138,7 +155,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + col * 8;
   T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + col * 8;
   const long long q0 = (long long)blockIdx.x * p.ppblock, q1 = min(q0 + p.ppblock, (long long)p.HW);
-  constexpr int U = 2;                                  // loads in flight a thread (1: 77.5 us, 2: 78.5 / 66.0, 4: 86.4 / 69.9 at 4x360x640x64 fp16 / 2x270x480x96 fp32)
+  constexpr int U = 2;                                  // loads in flight a thread (at 4x360x640x64 fp16 / 2x270x480x96 fp32: 1: 77.5 / 66.6 us, 2: 78.5 / 66.0, 4: 86.4 / 69.9)
   for (long long q = q0 + pr; q < q1; q += U * rows) {
     float v[U][8];
 #pragma unroll
@@ -150,7 +167,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = fmaf(v[u][i] - mean[i], mul[i], add[i]);
         act_values<8>(v[u], p.act, p.act_param);
-        store8<T>(y + (q + u * rows) * p.out_cs, v[u]);
+        if constexpr (STREAM) stream8<T>(y + (q + u * rows) * p.out_cs, v[u]);
+        else store8<T>(y + (q + u * rows) * p.out_cs, v[u]);
       }
   }
 }
@@ -230,7 +248,7 @@ __global__ __launch_bounds__(BLOCK) void gn_group_kernel(const GnParams p) {
 
 using namespace pp;
 
-// A group in one block's registers where it fits: 30 x 54 x 128 in 8 groups ONEFIG us in one launch, 11.7 in two.
+// A group in one block's registers where it fits: 30 x 54 x 128 in 8 groups 6.5 us in one launch, 11.7 in two.
 static int gn_group_block(int64_t HW, int C, int groups) {      // threads, 0: it does not fit
   const int cg = C / groups;
   if (cg % 8 != 0) return 0;
@@ -299,12 +317,16 @@ extern "C" int pp_group_norm(const void* in, int in_cstride, int in_choff, void*
   if (blocks > most) blocks = most;
   p.ppblock = ceil_div(HW, blocks);
   blocks = ceil_div(HW, p.ppblock);
+  // maps of 64 MB and more: 4x360x640x64 fp16 75 us against 86, 2x270x480x96 fp32 67 against 75; smaller outputs stay in the cache for their reader
+  const bool past = (int64_t)N * HW * C * (dtype == PP_F16 ? 2 : 4) >= (64 << 20);
   if (dtype == PP_F16) {
     hipLaunchKernelGGL((gn_stats_kernel<_Float16>), dim3(p.slices, N), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((gn_apply_kernel<_Float16>), dim3(blocks, N), dim3(256), 0, st, p);
+    if (past) hipLaunchKernelGGL((gn_apply_kernel<_Float16, true>), dim3(blocks, N), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((gn_apply_kernel<_Float16, false>), dim3(blocks, N), dim3(256), 0, st, p);
   } else {
     hipLaunchKernelGGL((gn_stats_kernel<float>), dim3(p.slices, N), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((gn_apply_kernel<float>), dim3(blocks, N), dim3(256), 0, st, p);
+    if (past) hipLaunchKernelGGL((gn_apply_kernel<float, true>), dim3(blocks, N), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((gn_apply_kernel<float, false>), dim3(blocks, N), dim3(256), 0, st, p);
   }
   return launch_status("pp_group_norm");
 }
