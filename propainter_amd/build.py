@@ -26,6 +26,9 @@ STAMP_PATH = os.path.join(LIB_DIR, "build_stamp.txt")
 # now and then; the scalar instructions round alike, so results are unchanged (the host pass warns that it does not know the feature)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# These round a product to fp32 before they round it to fp16, as they did while their products were packed: without the packed instructions hipcc
+# would merge the two roundings into v_fma_mixlo_f16.
+FILE_FLAGS = {name: ["-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"] for name in ("conv_gemm_v2s.hip", "conv_gemm_v3.hip", "conv_gemm_v3s.hip")}
 if os.environ.get("PP_DIAG") == "1":       # tuning builds: compiles the diagnostic / ablation kernel variants tools/kbench and
     FLAGS.append("-DPP_DIAG")            # tools/bench_dcn.py select through pp_conv_args_t.impl (never in the shipped library)
 
@@ -43,7 +46,7 @@ def _hipcc():
 
 
 def source_digest():
-    h = hashlib.sha256(" ".join(FLAGS).encode())
+    h = hashlib.sha256((" ".join(FLAGS) + str(sorted(FILE_FLAGS.items()))).encode())
     deps = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.h")) +
                   glob.glob(os.path.join(INCLUDE, "*.h")))
     for d in deps:
@@ -88,6 +91,7 @@ def build(force=False, verbose=True):
                 procs, objs = [], []
                 for s in sources():
                     h = hdr.copy()
+                    h.update(" ".join(FILE_FLAGS.get(s, [])).encode())
                     with open(os.path.join(CSRC, s), "rb") as f:
                         h.update(f.read())
                     obj = os.path.join(cache, f"{s[:-4]}.{h.hexdigest()[:16]}.o")
@@ -97,7 +101,7 @@ def build(force=False, verbose=True):
                     for old in glob.glob(os.path.join(cache, f"{s[:-4]}.*.o")):
                         os.unlink(old)
                     obj_tmp = os.path.join(tmp, s.replace(".hip", ".o"))
-                    cmd = [hipcc] + FLAGS + ["-c", os.path.join(CSRC, s), "-o", obj_tmp]
+                    cmd = [hipcc] + FLAGS + FILE_FLAGS.get(s, []) + ["-c", os.path.join(CSRC, s), "-o", obj_tmp]
                     procs.append((s, obj_tmp, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
                 errors = []
                 for s, obj_tmp, obj, p in procs:

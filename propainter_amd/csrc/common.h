@@ -177,6 +177,15 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 // overflow anywhere in the split-plane engine reaches the flows as NaN and RAFT_bi's finite-flow guard reports it.
 __device__ __forceinline__ float relu_split(float v) { return v > 0.f ? v : v * 0.f; }
 
+// The fp32 value itself.  Where v is a product, hipcc may round it to fp16 together with the multiplication (v_fma_mixlo_f16: one rounding) for
+// one use and in two roundings for another; a split needs ONE hi, or its lo belongs to a neighbour.
+__device__ __forceinline__ float settled(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(v));
+#endif
+  return v;
+}
+
 // Split-plane ("f16x3") store: hi = fp16(v), lo = fp16(v - hi); hi + lo carries 22 significand bits of v (|v| < 65504).
 __device__ __forceinline__ void store8_split(_Float16* hi_p, _Float16* lo_p, const float* v) {
   u32x4 rh, rl;
@@ -184,8 +193,9 @@ __device__ __forceinline__ void store8_split(_Float16* hi_p, _Float16* lo_p, con
   _Float16* l = reinterpret_cast<_Float16*>(&rl);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    h[i] = (_Float16)v[i];
-    l[i] = (_Float16)(v[i] - (float)h[i]);
+    const float x = settled(v[i]);
+    h[i] = (_Float16)x;
+    l[i] = (_Float16)(x - (float)h[i]);
   }
   *reinterpret_cast<u32x4*>(hi_p) = rh;
   *reinterpret_cast<u32x4*>(lo_p) = rl;

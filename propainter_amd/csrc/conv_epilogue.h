@@ -300,9 +300,10 @@ __device__ __forceinline__ void conv_epilogue(const ConvParams& p, f32x4 (&acc_)
 #pragma unroll
             for (int r = 0; r < 8; ++r)
               if (r < nval) {
-                const _Float16 h = (_Float16)v[r];
+                const float x = settled(v[r]);
+                const _Float16 h = (_Float16)x;
                 op[r] = h;
-                op[r + p.out_lo] = (_Float16)(v[r] - (float)h);
+                op[r + p.out_lo] = (_Float16)(x - (float)h);
               }
           }
         } else if (nval == 8 && ((p.out_cstride | out_cbase) & 7) == 0) store8<_Float16>(op, v);

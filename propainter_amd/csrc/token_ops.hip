@@ -397,7 +397,7 @@ __global__ void nchw_to_nhwc_split_kernel(const float* __restrict__ in, _Float16
     const int p = (int)(i % HW);
     const int c = (int)((i / HW) % C);
     const long long n = i / ((long long)HW * C);
-    const float v = in[i] * scale;
+    const float v = settled(in[i] * scale);
     const _Float16 hi = (_Float16)v;
     out[(n * HW + p) * ocs + oco + c] = hi;
     out[(n * HW + p) * ocs + ocs / 2 + oco + c] = (_Float16)(v - (float)hi);
