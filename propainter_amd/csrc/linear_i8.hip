@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ __attribute__((aligned(1024))) char lds[2 * 4 * KT * 1024];
   __shared__ float xs[2][64];                      // scales of the tile's tokens
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // (scalar branches on it)
   const int panel = (int)(blockIdx.x >> 3) % panels, grp = (int)(blockIdx.x >> 3) / panels * 8 + (int)(blockIdx.x & 7);
   const int nb = panel * 4 + wave, last = (p.N + 63) / 64 - 1;
   i32x4 wf[KT][4];

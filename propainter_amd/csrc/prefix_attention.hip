@@ -729,7 +729,17 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
   };
   if (packed && a->S > 0) {
     add(1, 0, 1, PA_SLOTS, true);
-    add(nseq, 1, 0, PA_SLOTS / 2, true);
+    // Blocks for the packed rows: every split leaves outputs to join, and their blocks take the place of suffix walks, so no more than finish their
+    // products while the suffixes (taken as half full) come out of memory, and at most one a CU.  A tile's products take about 2 us (two fp16
+    // row tiles of 16; fp32 four times that), the suffixes come at 4.3 TB/s.  Against 256 always (us): 64 sequences behind 8192 keys, suffixes up to
+    // 1024: 54 / 64.5, behind 2048: 46 / 50; 16 sequences behind 32768 keys, suffixes up to 512, where 128 blocks are too few: 50 with 256, 71.5.
+    const long long prows = R * nseq;
+    const long long units = ((prows + 63) / 64) * a->G * a->Hkv * ceil_div(a->P, 64) * (esz == 2 ? 1 : 4);      // us of products
+    const long long suffix = (long long)a->B * a->Hkv * a->S * a->D * esz / 4300000 + 1;                        // us of half of the suffix bytes
+    long long most = (units + suffix - 1) / suffix;
+    if (most < 32) most = 32;
+    if (most > PA_SLOTS / 2) most = PA_SLOTS / 2;
+    add(nseq, 1, 0, (int)most, true);
   } else if (packed) {
     add(nseq, 1, 0, PA_SLOTS, false);
   } else {
