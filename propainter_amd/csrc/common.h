@@ -177,6 +177,19 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float* 
 // overflow anywhere in the split-plane engine reaches the flows as NaN and RAFT_bi's finite-flow guard reports it.
 __device__ __forceinline__ float relu_split(float v) { return v > 0.f ? v : v * 0.f; }
 
+// 16 bytes from or to any address (global memory takes unaligned accesses: one instruction)
+__device__ __forceinline__ u32x4 load16_any(const void* p) {
+  u32x4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store8_any(T* p, const float* v) {
+  T r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (T)v[i];
+  __builtin_memcpy(p, r, 8 * sizeof(T));
+}
+
 // The fp32 value itself.  Where v is a product, hipcc may round it to fp16 together with the multiplication (v_fma_mixlo_f16: one rounding) for
 // one use and in two roundings for another; a split needs ONE hi, or its lo belongs to a neighbour.
 __device__ __forceinline__ float settled(float v) {

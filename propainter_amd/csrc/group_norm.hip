@@ -33,11 +33,28 @@ __device__ __forceinline__ void chan_merge(float& n, float& m, float& M2, float 
   n = nt;
 }
 
+// Threads s0 = 0 .. per - 1 hold parts of one group (thread s0 * ng + g of group g): joined into thread g, in a fixed order.  All threads call it.
+__device__ __forceinline__ void join_parts(int per, int ng, int s0, float& cnt, float& m, float& M2, float (*lds)[256]) {
+  const int t = threadIdx.x;
+  lds[0][t] = cnt; lds[1][t] = m; lds[2][t] = M2;
+  for (int h = per; h > 1;) {
+    const int half = (h + 1) >> 1;
+    __syncthreads();
+    if (s0 < h - half) {
+      const int o = t + half * ng;
+      chan_merge(cnt, m, M2, lds[0][o], lds[1][o], lds[2][o]);
+      lds[0][t] = cnt; lds[1][t] = m; lds[2][t] = M2;
+    }
+    h = half;
+  }
+  __syncthreads();
+}
+
 // 256 threads: column = 8 channels, the rest of the block walks the pixels of one slice.  Sums are taken relative to the slice's first
 // pixel (per channel), so that they hold deviations and not magnitudes.
 template <typename T>
 __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
-  __shared__ float s1[256 * 8], s2[256 * 8];
+  __shared__ float s1[256 * 8], s2[256 * 8], parts[3][256];
   const int c8 = p.C >> 3, rows = 256 / c8;
   const int t = threadIdx.x, col = t % c8, pr = t / c8;
   const bool on = pr < rows;
@@ -84,12 +101,18 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
     s1[c] = to_f32(x0[c]) + m;
   }
   __syncthreads();
-  for (int g = t; g < p.groups; g += 256) {
+  const int per = p.groups < 256 ? 256 / p.groups : 1;   // threads that share one group's channels
+  for (int g0 = 0; g0 < p.groups; g0 += 256) {
+    const int ng = min(256, p.groups - g0), g = g0 + t % ng, s0 = t / ng;
     float cnt = 0.f, m = 0.f, M2 = 0.f;
-    for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) chan_merge(cnt, m, M2, (float)np, s1[c], s2[c]);
-    float* o = p.part + (((long long)n * p.slices + slice) * p.groups + g) * 2;
-    o[0] = m;
-    o[1] = M2;
+    if (s0 < per)
+      for (int c = s0; c < p.cg; c += per) chan_merge(cnt, m, M2, (float)np, s1[g * p.cg + c], s2[g * p.cg + c]);
+    join_parts(per, ng, s0, cnt, m, M2, parts);
+    if (s0 == 0) {
+      float* o = p.part + (((long long)n * p.slices + slice) * p.groups + g) * 2;
+      o[0] = m;
+      o[1] = M2;
+    }
   }
 }
 
@@ -111,7 +134,7 @@ template <typename T> __device__ __forceinline__ void stream8(T* p, const float*
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   __shared__ float gm[2048], gr[2048];                 // mean and rstd of every group (groups <= C <= 2048)
-  __shared__ float part_n[256], part_m[256], part_v[256];
+  __shared__ float parts[3][256];
   const int t = threadIdx.x, n = blockIdx.y;
   const float* part = p.part + (long long)n * p.slices * p.groups * 2;
   const int per = p.groups < 256 ? 256 / p.groups : 1;  // threads that share one group's slices
@@ -125,17 +148,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
         const float* e = part + ((long long)s * p.groups + g0 + g) * 2;
         chan_merge(cnt, m, M2, (float)np * (float)p.cg, e[0], e[1]);
       }
-    part_n[t] = cnt; part_m[t] = m; part_v[t] = M2;
-    for (int h = per; h > 1;) {
-      const int half = (h + 1) >> 1;
-      __syncthreads();
-      if (s0 < h - half) {
-        const int o = t + half * ng;
-        chan_merge(cnt, m, M2, part_n[o], part_m[o], part_v[o]);
-        part_n[t] = cnt; part_m[t] = m; part_v[t] = M2;
-      }
-      h = half;
-    }
+    join_parts(per, ng, s0, cnt, m, M2, parts);
     if (s0 == 0) {
       gm[g0 + g] = m;
       gr[g0 + g] = 1.f / sqrtf(M2 / cnt + p.eps);

@@ -18,17 +18,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------------------------------------------------------------
 // codes of token rows
 // ---------------------------------------------------------------------------------------------------------------------------------
-// 8 elements at column c of a row of K; columns past K are 0.  `wide`: rows are 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void row_load8(const T* row, int c, int K, bool wide, float* v) {
-  if (wide && c + 8 <= K) {
-    load8<T>(row + c, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.f;
-  }
-}
-
 // |v| as ordered bits: the maximum of these keeps NaN (largest) and infinity, which fmaxf would drop
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
@@ -125,7 +114,12 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 template <> struct Raw8<_Float16> {
   u32x4 r;
   __device__ __forceinline__ void load(const _Float16* p) { r = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void load_any(const _Float16* p) { r = load16_any(p); }
   __device__ __forceinline__ void clear() { r = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void keep(int n) {            // elements n .. 7 become 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = 2 * i + 1 < n ? r[i] : 2 * i < n ? r[i] & 0xffffu : 0u;
+  }
   __device__ __forceinline__ void set(int i, _Float16 v) {
     const unsigned u = __builtin_bit_cast(unsigned short, v);
     r[i >> 1] = (i & 1) ? (r[i >> 1] & 0xffffu) | (u << 16) : (r[i >> 1] & 0xffff0000u) | u;
@@ -146,7 +140,12 @@ template <> struct Raw8<_Float16> {
 template <> struct Raw8<float> {
   u32x4 r[2];
   __device__ __forceinline__ void load(const float* p) { r[0] = *reinterpret_cast<const u32x4*>(p); r[1] = *reinterpret_cast<const u32x4*>(p + 4); }
+  __device__ __forceinline__ void load_any(const float* p) { r[0] = load16_any(p); r[1] = load16_any(p + 4); }
   __device__ __forceinline__ void clear() { r[0] = r[1] = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void keep(int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i >> 2][i & 3] = i < n ? r[i >> 2][i & 3] : 0u;
+  }
   __device__ __forceinline__ void set(int i, float v) { r[i >> 2][i & 3] = __float_as_uint(v); }
   __device__ __forceinline__ void values(float* v) const {
 #pragma unroll
@@ -171,6 +170,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, lon
   for (long long row0 = blockIdx.x * (long long)(4 / WPR); row0 < rows; row0 += gridDim.x * (long long)(4 / WPR)) {
     const long long row = row0 + wave / WPR;
     const T* xr = x + min(row, rows - 1) * xrs;
+    const bool inside = row < rows - 1 && xrs >= 8;        // a vector past this row's end is still inside the rows
     Raw8<T> raw[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
@@ -178,6 +178,9 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, lon
       if constexpr (WIDE) {
         raw[v].load(xr + (c < K ? c : 0));
         if (c >= K) raw[v].clear();
+      } else if (c + 8 <= K || (c < K && inside)) {
+        raw[v].load_any(xr + c);
+        raw[v].keep(K - c);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < K ? xr[c + i] : (T)0.f);
@@ -212,28 +215,34 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, lon
 // One block of 256 threads per row, any K: the row is read twice (the second time from L2).
 template <typename T>
 __global__ __launch_bounds__(256) void quant_row_kernel(const T* __restrict__ x, long long xrs, int8_t* __restrict__ q, long long qrs,
-                                                        float* __restrict__ scale, long long rows, int K, int Kp, int wide) {
+                                                        float* __restrict__ scale, long long rows, int K, int Kp) {
   __shared__ unsigned wm[4];
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-  const T* xr = x + row * xrs;
-  unsigned m = 0;
-  for (int c = threadIdx.x * 8; c < K; c += 2048) {
-    float v[8];
-    row_load8<T>(xr, c, K, wide, v);
+  auto vector = [&](const T* xr, int c) {
+    Raw8<T> raw;
+    if (c + 8 <= K) {
+      raw.load_any(xr + c);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
-  }
-  m = wave_umax(m);
-  if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
-  __syncthreads();
-  const RowScale r = row_scale(max(max(wm[0], wm[1]), max(wm[2], wm[3])));
-  if (threadIdx.x == 0) scale[row] = r.scale;
-  for (int c = threadIdx.x * 8; c < Kp; c += 2048) {
-    float v[8];
-    row_load8<T>(xr, c, K, wide, v);
-    *reinterpret_cast<u32x2*>(q + row * qrs + c) = codes8(v, r);
-  }
-  __syncthreads();
+      for (int i = 0; i < 8; ++i) raw.set(i, c + i < K ? xr[c + i] : (T)0.f);
+    }
+    return raw;
+  };
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * xrs;
+    unsigned m = 0;
+    for (int c = threadIdx.x * 8; c < K; c += 2048) m = max(m, vector(xr, c).amax());
+    m = wave_umax(m);
+    if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const RowScale r = row_scale(max(max(wm[0], wm[1]), max(wm[2], wm[3])));
+    if (threadIdx.x == 0) scale[row] = r.scale;
+    const float half = !r.zero && r.lift == 1.f ? 0.5f * r.s : -1.f;
+    for (int c = threadIdx.x * 8; c < Kp; c += 2048) {
+      float f[8];
+      vector(xr, c).values(f);
+      *reinterpret_cast<u32x2*>(q + row * qrs + c) = codes8_fast(f, r, half);
+    }
+    __syncthreads();
   }
 }
 
@@ -273,7 +282,6 @@ struct LinI8Params {
   long long qrs, ors, M;
   int N, ktiles, act;
   float act_param;
-  int wide_out;      // rows of `out` are 16-byte aligned
 };
 
 // 8 consecutive channels c .. c + 7 that a lane holds of two neighbouring operand tiles, with their scales and biases
@@ -297,8 +305,8 @@ template <typename TO> struct Lane8 {
   }
   __device__ __forceinline__ void store(const LinI8Params& p, long long m, const float* v) const {
     TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c;
-    if (p.wide_out && c + 8 <= p.N) {
-      store8<TO>(o, v);
+    if (c + 8 <= p.N) {
+      store8_any<TO>(o, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -310,7 +318,7 @@ template <typename TO> struct Lane8 {
 // Few tokens: the weights' bytes are the work.  A block takes TPB operand tiles (16 channels each) of one 64-channel block and 16 MT tokens; its 8
 // waves share out K, operands straight from memory, several tiles in flight, and add their exact partial sums through LDS.
 constexpr int I8_KW = 8;
-template <typename T> struct FloatTokens { const T* x; long long xrs; int K, wide; };
+template <typename T> struct FloatTokens { const T* x; long long xrs; int K; };
 
 // acc[t][j] += tiles kt0 .. kt1 of the weights times the tokens; tok(kt, j) gives the token operand
 template <int MT, int TPB, typename F>
@@ -415,8 +423,8 @@ __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, 
     if (v >= M * per) break;
     const T* xr = x.x + (long long)(v / per) * x.xrs;
     const int c = v % per * 4096 + threadIdx.x * 8;
-    if (x.wide && c + 8 <= x.K) {
-      raw[v].load(xr + c);
+    if (c + 8 <= x.K) {
+      raw[v].load_any(xr + c);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < x.K ? xr[c + i] : (T)0.f);
@@ -604,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                  // tile is there for all waves; the other stage, read one tile ago, is free
     if (tile + groups < tiles) issue(tile + groups, buf ^ 1);
-    full = p.wide_out && nb * 64 + 64 <= p.N && tile * 64ll + 64 <= p.M;
+    full = nb * 64 + 64 <= p.N && tile * 64ll + 64 <= p.M;
     const char* st = lds + buf * 4 * KT * 1024 + lane * 16;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -623,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params
       for (int h = 0; h < 2; ++h) {
         float v[8];
         ch[h].value(p, xm, &acc[h * 2], v);
-        if (full) store8<TO>(reinterpret_cast<TO*>(p.out) + m * p.ors + ch[h].c, v);
+        if (full) store8_any<TO>(reinterpret_cast<TO*>(p.out) + m * p.ors + ch[h].c, v);
         else if (m < p.M) ch[h].store(p, m, v);
       }
     }
@@ -700,7 +708,7 @@ static void launch_quant(const void* x, int64_t xrs, void* q, int64_t qrs, float
   else if (K <= 4096) PP_QUANT(2, 4);
   else if (K <= 8192) PP_QUANT(4, 4);
   else if (K <= 16384) PP_QUANT(8, 4);
-  else hipLaunchKernelGGL((quant_row_kernel<T>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp, wide);
+  else hipLaunchKernelGGL((quant_row_kernel<T>), grid, block, 0, st, (const T*)x, (long long)xrs, (int8_t*)q, (long long)qrs, scale, (long long)rows, K, Kp);
 #undef PP_QUANT
 #undef PP_QUANT_FORM
 }
@@ -750,11 +758,10 @@ static int lin_i8_check(const char* who, const void* weight, const float* ws, co
   return 0;
 }
 static LinI8Params lin_i8_params(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out, int64_t out_rstride,
-                                 int64_t M, int N, int K, int act, float act_param, int out_dtype) {
+                                 int64_t M, int N, int K, int act, float act_param) {
   LinI8Params p;
   p.xq = (const int8_t*)xq; p.xs = xs; p.w = (const u32x4*)weight; p.ws = ws; p.bias = bias; p.out = (char*)out;
   p.qrs = q_rstride; p.ors = out_rstride; p.M = M; p.N = N; p.ktiles = pp_i8_row_bytes(K) / 64; p.act = act; p.act_param = act_param;
-  p.wide_out = (uintptr_t)out % 16 == 0 && out_rstride * (out_dtype == PP_F16 ? 2 : 4) % 16 == 0;
   return p;
 }
 
@@ -765,7 +772,7 @@ extern "C" int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, 
   const int Kp = pp_i8_row_bytes(K);
   PP_REQUIRE(xq && xs && q_rstride >= Kp, PP_ERR_ARG, "pp_linear_i8: null codes or row stride (%lld < %d)", (long long)q_rstride, Kp);
   PP_REQUIRE((uintptr_t)xq % 16 == 0 && q_rstride % 16 == 0, PP_ERR_ALIGN, "pp_linear_i8: codes and their row stride must be multiples of 16 bytes");
-  const LinI8Params p = lin_i8_params(xq, q_rstride, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype);
+  const LinI8Params p = lin_i8_params(xq, q_rstride, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param);
   if (out_dtype == PP_F16) launch_product<_Float16>(p, (hipStream_t)stream);
   else launch_product<float>(p, (hipStream_t)stream);
   return launch_status("pp_linear_i8");
@@ -796,10 +803,9 @@ extern "C" int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype
     if ((rc = pp_quantize_tokens(x, x_rstride, q, Kp, xs, M, K, x_dtype, stream)) != 0) return rc;
     return pp_linear_i8(q, Kp, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype, stream);
   }
-  const LinI8Params p = lin_i8_params(nullptr, 0, nullptr, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype);
-  const int wide = (uintptr_t)x % 16 == 0 && x_rstride * esz % 16 == 0;
+  const LinI8Params p = lin_i8_params(nullptr, 0, nullptr, weight, ws, bias, out, out_rstride, M, N, K, act, act_param);
   const dim3 grid((unsigned)((N + 63) / 64 * 4)), block(512);
-#define PP_TOKEN(T, TO) hipLaunchKernelGGL((lin_i8_token_kernel<T, TO>), grid, block, 0, (hipStream_t)stream, p, FloatTokens<T>{(const T*)x, (long long)x_rstride, K, wide})
+#define PP_TOKEN(T, TO) hipLaunchKernelGGL((lin_i8_token_kernel<T, TO>), grid, block, 0, (hipStream_t)stream, p, FloatTokens<T>{(const T*)x, (long long)x_rstride, K})
   if (x_dtype == PP_F16) { if (out_dtype == PP_F16) PP_TOKEN(_Float16, _Float16); else PP_TOKEN(_Float16, float); }
   else { if (out_dtype == PP_F16) PP_TOKEN(float, _Float16); else PP_TOKEN(float, float); }
 #undef PP_TOKEN

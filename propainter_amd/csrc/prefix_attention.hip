@@ -298,16 +298,39 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     if (t + 1 < t1) load_tile(t + 1);
     // ---- scores: sacc[qt][kt][r] = key wkey + kt * 16 + lg * 4 + r, query lc of row tile qt
     f32x4 sacc[QT][NK];
-#pragma unroll
-    for (int kt = 0; kt < NK; ++kt) {
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto key_frag = [&](int kt, int st) {
       const int key = wkey + kt * 16 + lc;
+      return *reinterpret_cast<const frag*>(&Ks[key * D + ((st * 4 + lg) ^ swz(key)) * (16 / sizeof(T))]);
+    };
+    if constexpr (C::F16) {
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const frag kf = *reinterpret_cast<const frag*>(&Ks[key * D + ((s * 4 + lg) ^ swz(key)) * (16 / sizeof(T))]);
+      for (int kt = 0; kt < NK; ++kt) {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = PaOps<T>::mfma(kf, qf[qt][s], sacc[qt][kt]);
+        for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+          const frag kf = key_frag(kt, st);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = PaOps<T>::mfma(kf, qf[qt][st], sacc[qt][kt]);
+        }
+      }
+    } else {
+      // fp32 products take twice as long and leave registers: the next operand is requested ahead of this one's products
+      frag cur = key_frag(0, 0);
+#pragma unroll
+      for (int i = 0; i < NK * STEPS; ++i) {
+        const int kt = i / STEPS, st = i % STEPS;
+        frag next = cur;
+        if (i + 1 < NK * STEPS) next = key_frag((i + 1) / STEPS, (i + 1) % STEPS);
+        __builtin_amdgcn_sched_barrier(0);
+        if (st == 0)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur[j], (float)qf[qt][st][j], sacc[qt][kt], 0, 0, 0);
+        cur = next;
       }
     }
     // ---- online softmax in the exp2 domain
@@ -372,16 +395,22 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     } else {
       // one key a lane group: slot lg is key kt * 16 + lg * 4 + r; accumulator row i of tile d is channel d * 16 + i
       const float* vb = reinterpret_cast<const float*>(Vs) + (wkey + lg * 4) * C::VLD + lc;
+      float cur[DT], next[DT];
 #pragma unroll
-      for (int kt = 0; kt < NK; ++kt)
+      for (int d = 0; d < DT; ++d) cur[d] = vb[d * 16];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int i = 0; i < NK * 4; ++i) {
+        if (i + 1 < NK * 4)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const float vv = vb[(kt * 16 + r) * C::VLD + d * 16];
+          for (int d = 0; d < DT; ++d) next[d] = vb[((i + 1) / 4 * 16 + (i + 1) % 4) * C::VLD + d * 16];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, sacc[qt][kt][r], oacc[qt][d], 0, 0, 0);
-          }
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) oacc[qt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur[d], sacc[qt][i / 4][i % 4], oacc[qt][d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) cur[d] = next[d];
+      }
     }
     __syncthreads();
   }
