@@ -402,67 +402,65 @@ __global__ __launch_bounds__(512) void lin_i8_thin_kernel(const LinI8Params p) {
   thin_finish<TO, MT, TPB>(p, red, acc, nb, t0, m0, [&](long long m) { return p.xs[m]; });
 }
 
-// One or two float tokens (M * ceil(K / 4096) <= 2): every block makes their codes itself, into LDS -- they come out of L2, and a launch and a
-// round trip of the codes are saved.  4096 -> 4096: one token 8.0 us against 7.0 for the product alone plus a launch for the codes; four tokens
-// 10.4, no gain any more.
-constexpr int I8_FUSE = 2;
-inline bool i8_fused(int64_t M, int K) { return M * ((K + 4095) / 4096) <= I8_FUSE; }
+// Few float tokens (at most 16, 2048 vectors of 8 in all): every block makes their codes itself, into LDS -- they come out of L2, and a launch and a
+// round trip of the codes are saved.  4096 -> 4096: one token 8.0 us against 7.0 for the product alone plus a launch for the codes, four
+// tokens 10.4 against 7.2 plus that launch.
+constexpr int I8_FUSE_VEC = 4;                     // vectors a thread
+inline bool i8_fused(int64_t M, int K) { return M <= 16 && M * ((K + 63) / 64 * 8) <= 512 * I8_FUSE_VEC; }
 template <typename T, typename TO>
 __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, const FloatTokens<T> x) {
-  constexpr int TPB = 1;
-  __shared__ __attribute__((aligned(16))) i32x4 red[TPB * I8_KW * 64];
-  __shared__ __attribute__((aligned(16))) int8_t codes[I8_FUSE * (4096 + 16)];
-  __shared__ unsigned wmax[I8_FUSE][8];
-  __shared__ float xs[I8_FUSE];
+  __shared__ __attribute__((aligned(16))) i32x4 red[I8_KW * 64];
+  __shared__ __attribute__((aligned(16))) int8_t codes[512 * I8_FUSE_VEC * 8 + 16 * 16];       // rows of K padded to 64, 16 bytes apart
+  __shared__ unsigned rmax[16];
+  __shared__ float xs[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nb = blockIdx.x / (4 / TPB), t0 = blockIdx.x % (4 / TPB) * TPB;
-  const int M = (int)p.M, Kp = p.ktiles * 64, per = (x.K + 4095) / 4096, ld = per * 4096 + 16;      // M * ld <= sizeof(codes)
-  Raw8<T> raw[I8_FUSE];                            // vector v = token v / per, columns (v % per) * 4096 + thread * 8 ..
+  const int nb = blockIdx.x >> 2, t0 = blockIdx.x & 3;
+  const int M = (int)p.M, Kp = p.ktiles * 64, vr = Kp >> 3, ld = Kp + 16;
+  if (threadIdx.x < 16) rmax[threadIdx.x] = 0;
+  __syncthreads();
+  Raw8<T> raw[I8_FUSE_VEC];
+  int row[I8_FUSE_VEC];
 #pragma unroll
-  for (int v = 0; v < I8_FUSE; ++v) {
-    if (v >= M * per) break;
-    const T* xr = x.x + (long long)(v / per) * x.xrs;
-    const int c = v % per * 4096 + threadIdx.x * 8;
-    if (c + 8 <= x.K) {
-      raw[v].load_any(xr + c);
-    } else {
+  for (int v = 0; v < I8_FUSE_VEC; ++v) {
+    const int i = v * 512 + threadIdx.x, r = i / vr, c = (i - r * vr) * 8;
+    row[v] = r < M ? r : -1;
+    raw[v].clear();
+    if (row[v] >= 0 && c < x.K) {
+      const T* xr = x.x + (long long)r * x.xrs + c;
+      if (c + 8 <= x.K) {
+        raw[v].load_any(xr);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) raw[v].set(i, c + i < x.K ? xr[c + i] : (T)0.f);
+        for (int k = 0; k < 8; ++k)
+          if (c + k < x.K) raw[v].set(k, xr[k]);
+      }
     }
   }
 #pragma unroll
-  for (int v = 0; v < I8_FUSE; ++v) {
-    if (v >= M * per) break;
-    const unsigned m = wave_umax(raw[v].amax());
-    if (lane == 0) wmax[v][wave] = m;
+  for (int v = 0; v < I8_FUSE_VEC; ++v) {
+    unsigned m = raw[v].amax();                    // 8 neighbouring lanes hold one row: vr is a multiple of 8
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    if ((lane & 7) == 0 && row[v] >= 0) atomicMax(&rmax[row[v]], m);      // (a maximum: the order does not matter)
   }
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < I8_FUSE; ++v) {
-    if (v >= M * per) break;
-    const int row = v / per;
-    unsigned m = 0;
-    for (int k = row * per; k < (row + 1) * per; ++k)
-#pragma unroll
-      for (int w = 0; w < 8; ++w) m = max(m, wmax[k][w]);
-    m = __builtin_amdgcn_readfirstlane(m);
-    const RowScale r = row_scale(m);
-    if (threadIdx.x == 0) xs[row] = r.scale;
-    const int c = v % per * 4096 + threadIdx.x * 8;
+  for (int v = 0; v < I8_FUSE_VEC; ++v) {
+    if (row[v] < 0) continue;
+    const int c = (v * 512 + threadIdx.x - row[v] * vr) * 8;
+    const RowScale r = row_scale(rmax[row[v]]);
+    if (c == 0) xs[row[v]] = r.scale;
     float f[8];
     raw[v].values(f);
-    if (c < Kp) *reinterpret_cast<u32x2*>(codes + row * ld + c) = codes8_fast(f, r, !r.zero && r.lift == 1.f ? 0.5f * r.s : -1.f);
+    *reinterpret_cast<u32x2*>(codes + row[v] * ld + c) = codes8_fast(f, r, !r.zero && r.lift == 1.f ? 0.5f * r.s : -1.f);
   }
   __syncthreads();
-  i32x4 acc[TPB][1];
-#pragma unroll
-  for (int t = 0; t < TPB; ++t) acc[t][0] = i32x4{0, 0, 0, 0};
+  i32x4 acc[1][1] = {{i32x4{0, 0, 0, 0}}};
   const u32x4* w = p.w + (long long)nb * p.ktiles * 256 + t0 * 64 + lane;
-  const bool on = (lane & 15) < M;
-  const int8_t* xa = codes + (on ? lane & 15 : 0) * ld + (lane >> 4) * 16;
-  thin_product<1, TPB>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
-                       [&](int kt, int) { return *reinterpret_cast<const i32x4*>(xa + kt * 64); });
-  thin_finish<TO, 1, TPB>(p, red, acc, nb, t0, 0, [&](long long m) { return xs[m]; });
+  const int8_t* xa = codes + ((lane & 15) < M ? lane & 15 : 0) * ld + (lane >> 4) * 16;        // (columns past M repeat row 0 and are not stored)
+  thin_product<1, 1>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
+                     [&](int kt, int) { return *reinterpret_cast<const i32x4*>(xa + kt * 64); });
+  thin_finish<TO, 1, 1>(p, red, acc, nb, t0, 0, [&](long long m) { return xs[m]; });
 }
 
 // Tiles of BM tokens x BN channels, WM x WN waves of BM / WM tokens x BN / WN channels.  Both operands go from memory into LDS without

@@ -732,7 +732,7 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
     t.nper = nper; t.prefix = prefix; t.suffix = suffix; t.by_row = both;
     t.rows = (int)(R * nper);
     r.wk[i] = t.rows <= 32;
-    r.qt[i] = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 ? 1 : 2;
+    r.qt[i] = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 || (esz == 4 && a->D == 128) ? 1 : 2;      // (fp32 heads of 128: two row tiles leave one block a CU)
     const int per = 16 * r.qt[i] * (r.wk[i] ? 1 : 4);
     t.rowblocks = ceil_div(t.rows, per);
     const long long items = (long long)(a->B / nper) * a->Hkv * t.rowblocks;
