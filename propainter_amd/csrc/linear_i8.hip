@@ -752,7 +752,7 @@ static int lin_i8_check(const char* who, const void* weight, const float* ws, co
   if (M == 0) return 0;
   PP_REQUIRE(weight && ws && out && out_rstride >= N, PP_ERR_ARG, "%s: null buffer or row stride (out %lld < %d)", who, (long long)out_rstride, N);
   PP_REQUIRE((uintptr_t)weight % 16 == 0 && (uintptr_t)out % (out_dtype == PP_F16 ? 2 : 4) == 0, PP_ERR_ALIGN, "%s: the weight must be 16-byte aligned", who);
-  PP_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= (1 << 23), PP_ERR_ARG, "%s: too many tiles (M=%lld N=%d)", who, (long long)M, N);
+  PP_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) < (1 << 23), PP_ERR_ARG, "%s: too many tiles (M=%lld N=%d)", who, (long long)M, N);
   return 0;
 }
 static LinI8Params lin_i8_params(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out, int64_t out_rstride,

@@ -62,25 +62,15 @@ __device__ __forceinline__ int clamp_len(const int* lens, int i, int most) {
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-template <typename T> struct PaOps;
-template <> struct PaOps<_Float16> {
-  typedef f16x8 frag;      // 16 bytes of a row: 8 consecutive channels
-  static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-};
-template <> struct PaOps<float> {
-  typedef f32x4 frag;      // 16 bytes of a row: 4 consecutive channels, one contraction slot of 4 products
-  static __device__ __forceinline__ f32x4 mfma(frag a, frag b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-};
+// 16 bytes of a row: 8 consecutive fp16 channels, or 4 of fp32, one contraction slot of 4 products
+template <typename T> struct PaFrag { typedef f16x8 type; };
+template <> struct PaFrag<float> { typedef f32x4 type; };
 #endif
 
 template <typename T, int D, bool WK> struct PaTile {
   static constexpr bool F16 = sizeof(T) == 2;
-  static constexpr int KT = F16 && WK ? 128 : 64;             // keys of a tile
-  static constexpr int NK = WK ? KT / 64 : 4;                 // 16-key tiles of a wave
+  static constexpr int KT = 64;                               // keys of a tile
+  static constexpr int NK = WK ? 1 : 4;                       // 16-key tiles of a wave
   static constexpr int SLOTS = D * (int)sizeof(T) / 16;       // 16-byte slots of a key row
   static constexpr int STEPS = SLOTS / 4;                     // fragments of a row
   static constexpr int VLD = F16 ? D : D + 16;                // V row stride (elements); fp16 rows are swizzled (v_at), fp32 rows skewed
@@ -189,13 +179,14 @@ __device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& p
 #endif
 }
 
-// block `bid` of part `pt`
+// block `bid` of part `pt`, key tiles of 64 through LDS (fp16: WK = false alone, few rows go to pa_stream_block)
 template <typename T, int D, int QT, bool WK>
 __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, const int bid, char* lds, float* wave_ml) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef PaTile<T, D, WK> C;
-  typedef typename PaOps<T>::frag frag;
+  typedef typename PaFrag<T>::type frag;
   constexpr int KT = C::KT, NK = C::NK, STEPS = C::STEPS, DT = D / 16;
+  static_assert(!(C::F16 && WK), "fp16 blocks of few rows are streamed");
   T* Ks = reinterpret_cast<T*>(lds);
   T* Vs = reinterpret_cast<T*>(lds + C::KBYTES);
 
@@ -311,7 +302,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
         for (int st = 0; st < STEPS; ++st) {
           const frag kf = key_frag(kt, st);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = PaOps<T>::mfma(kf, qf[qt][st], sacc[qt][kt]);
+          for (int qt = 0; qt < QT; ++qt) sacc[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[qt][st], sacc[qt][kt], 0, 0, 0);
         }
       }
     } else {
@@ -336,7 +327,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
     // ---- online softmax in the exp2 domain
     const int n = tile_keys(t), j0 = (t - ptiles) * KT;
     const bool cut = p.causal && t >= ptiles && j0 + n > vis_min;      // rows of the block see different parts of the tile
-    constexpr int NP = C::F16 ? (NK + 1) / 2 : 1;
+    constexpr int NP = C::F16 ? NK / 2 : 1;
     f16x8 pfr[QT][NP];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -719,6 +710,9 @@ struct PaPlan {
 
 constexpr int PA_SLOTS = 512;         // blocks that run at a time: two a CU
 
+// two row tiles a wave where they leave two blocks a CU (fp32 heads of 128: 24 sequences of 413 queries over 77 + 622 keys 74 us with two, 50 with one)
+constexpr bool pa_two_row_tiles(int esz, int D) { return !(esz == 4 && D == 128); }
+
 inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
   PaPlan r{};
   r.ok = true;
@@ -732,7 +726,7 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
     t.nper = nper; t.prefix = prefix; t.suffix = suffix; t.by_row = both;
     t.rows = (int)(R * nper);
     r.wk[i] = t.rows <= 32;
-    r.qt[i] = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 || (esz == 4 && a->D == 128) ? 1 : 2;      // (fp32 heads of 128: two row tiles leave one block a CU)
+    r.qt[i] = t.rows <= 16 ? 1 : t.rows <= 32 ? 2 : t.rows <= 64 || !pa_two_row_tiles(esz, a->D) ? 1 : 2;
     const int per = 16 * r.qt[i] * (r.wk[i] ? 1 : 4);
     t.rowblocks = ceil_div(t.rows, per);
     const long long items = (long long)(a->B / nper) * a->Hkv * t.rowblocks;
@@ -781,6 +775,7 @@ inline int64_t pa_scratch(const PaPlan& plan, int D) { return plan.slots * plan.
 template <typename T, int D>
 static void pa_launch(const PaPlan& plan, const PaParams& p, hipStream_t st) {
   const dim3 block(256);
+  constexpr bool TWO = pa_two_row_tiles((int)sizeof(T), D);
   if (plan.nparts == 2) {
     const dim3 grid((unsigned)(plan.part[0].blocks + plan.part[1].blocks));
     const int form = plan.wk[1] ? plan.qt[1] - 1 : 1 + plan.qt[1];      // of the packed part: wk 1, wk 2, rows 1, rows 2; the suffix part is always wk
@@ -789,10 +784,10 @@ static void pa_launch(const PaPlan& plan, const PaParams& p, hipStream_t st) {
       if (form == 0) PA_PAIR(1, 1, true);
       else if (form == 1) PA_PAIR(1, 2, true);
       else if (form == 2) PA_PAIR(1, 1, false);
-      else PA_PAIR(1, 2, false);
+      else if constexpr (TWO) PA_PAIR(1, 2, false);
     } else {
       if (form == 2) PA_PAIR(2, 1, false);
-      else PA_PAIR(2, 2, false);
+      else if constexpr (TWO) PA_PAIR(2, 2, false);
     }
 #undef PA_PAIR
   } else {
@@ -802,7 +797,7 @@ static void pa_launch(const PaPlan& plan, const PaParams& p, hipStream_t st) {
       else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, true>), grid, block, 0, st, p);
     } else {
       if (plan.qt[0] == 1) hipLaunchKernelGGL((pa_tile_kernel<T, D, 1, false>), grid, block, 0, st, p);
-      else hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, false>), grid, block, 0, st, p);
+      else if constexpr (TWO) hipLaunchKernelGGL((pa_tile_kernel<T, D, 2, false>), grid, block, 0, st, p);
     }
   }
   if (plan.slots > 0)

@@ -801,6 +801,26 @@ def _raw_stream(who, x, *others):
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _refuse_overlap(who, out, *inputs):
+    """A given `out` may not share memory with what other blocks still read.  Views whose rows are the same stride apart may interleave
+    (columns of one buffer side by side)."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    for t in inputs:
+        if t is None or not t.numel() or not out.numel():
+            continue
+        (a0, a1), (b0, b1) = span(out), span(t)
+        if a1 <= b0 or b1 <= a0:
+            continue
+        if out.dim() == 2 and t.dim() == 2:
+            pitch = out.stride(0) * out.element_size()
+            shift = (b0 - a0) % pitch if pitch else 0
+            if pitch == t.stride(0) * t.element_size() and out.shape[1] * out.element_size() <= shift and shift + t.shape[1] * t.element_size() <= pitch:
+                continue
+        raise ValueError(f"{who}: out overlaps an input")
+
+
 @functools.lru_cache(maxsize=4096)
 def _group_norm_floats(N, H, W, Cc, groups):
     n = lib().pp_group_norm_workspace_floats(N, H, W, Cc, groups)
@@ -822,6 +842,7 @@ def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, act_par
         assert out.is_contiguous() and out.dtype == x.dtype and out.shape[:3] == x.shape[:3]
         if out.data_ptr() == x.data_ptr() and (out.shape != x.shape or out_choff != x_choff):
             raise ValueError("group_norm: in place needs the same channel window")
+        _refuse_overlap("group_norm", out, x if out.data_ptr() != x.data_ptr() else None, gamma, beta)
     stream = _raw_stream("group_norm", x, gamma, beta, out)
     assert x.is_contiguous()
     assert gamma is None or (gamma.dtype == torch.float32 and gamma.is_contiguous() and gamma.shape == (C_,))
@@ -905,13 +926,16 @@ def _linear_i8_out(who, weight, wscale, bias, N, K, M, dtype, out, device):
 
 def linear_i8(q, scale, weight, wscale, bias, N, K, act=ACT_NONE, act_param=0.0, out_dtype=torch.float16, out=None):
     """act(codes @ weight codes^T * scale * wscale + bias): q int8 [M, i8_row_bytes(K)], scale fp32 [M] (quantize_tokens), weight from
-    linear_i8_pack, wscale / bias fp32 [N] -> out [M, N] of out_dtype (or the first N columns of a given `out` [M, >= N])."""
+    linear_i8_pack, wscale / bias fp32 [N] -> out [M, N] of out_dtype (or the first N columns of a given `out` [M, >= N],
+    which may lie beside the inputs in one buffer but not over them)."""
     require_gpu(q, "linear_i8")
     M, Kp = q.shape[0], i8_row_bytes(K)
     if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous() or q.shape[1] != Kp:
         raise ValueError(f"linear_i8: codes must be int8 [M, {Kp}] as quantize_tokens returns them, got {q.dtype} {tuple(q.shape)}")
     if scale.dtype != torch.float32 or scale.shape != (M,) or not scale.is_contiguous():
         raise ValueError(f"linear_i8: scales must be float32 [{M}]")
+    if out is not None:
+        _refuse_overlap("linear_i8", out[:, :N], q, scale, weight, wscale, bias)
     out, ors = _linear_i8_out("linear_i8", weight, wscale, bias, N, K, M, out_dtype, out, q.device)
     stream = _raw_stream("linear_i8", q, scale, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
@@ -927,6 +951,8 @@ def linear_i8_tokens(x, weight, wscale, bias, N, act=ACT_NONE, act_param=0.0, ou
     require_gpu(x, "linear_i8_tokens")
     M, K, rs = _token_rows("linear_i8_tokens", x)
     xcode, Kp = dtype_code(x.dtype), i8_row_bytes(K)
+    if out is not None:
+        _refuse_overlap("linear_i8_tokens", out[:, :N], x, weight, wscale, bias)
     out, ors = _linear_i8_out("linear_i8_tokens", weight, wscale, bias, N, K, M, out_dtype or x.dtype, out, x.device)
     stream = _raw_stream("linear_i8_tokens", x, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
@@ -956,7 +982,7 @@ def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal
     q [B,Lq,Hq,D]; pk / pv [G,P,Hkv,D] or None; k / v [B,S,Hkv,D] or None; Hq a multiple of Hkv, D 64 or 128, fp16 or fp32, any strides with a
     contiguous last dimension.  Sequence b belongs to group b // (B // G).  prefix_lens int32 [G] / lens int32 [B] (device): the keys that
     count (default: all); causal: query i sees suffix keys up to lens[b] - Lq + i, and the values that causality hides from a query have to
-    be finite.  scale: default 1 / sqrt(D).  A query without keys gives zeros.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
+    be finite.  scale: default 1 / sqrt(D).  A query without keys gives zeros.  A given `out` may not overlap an input.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
     require_gpu(q, "shared_prefix_attention")
     B, Lq, Hq, D = qshape = q.shape
     dt = q.dtype
@@ -966,6 +992,8 @@ def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal
     S = k.shape[1] if k is not None else 0
     if out is None:
         out = torch.empty(qshape, dtype=dt, device=q.device)
+    else:
+        _refuse_overlap("shared_prefix_attention", out, q, pk, pv, k, v, prefix_lens, lens)
     stream = _raw_stream("shared_prefix_attention", q, pk, pv, k, v, prefix_lens, lens, out)
     pshape, kshape = (G, P, Hkv, D), (B, S, Hkv, D)
     packed = []

@@ -58,7 +58,8 @@ def make(shape, dtype, seed=0, shift=0.5):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("shape,groups", [((1, 1, 1, 8), 1), ((2, 1, 1, 64), 8), ((1, 5, 7, 24), 8), ((3, 9, 13, 40), 5), ((2, 30, 54, 128), 8), ((1, 33, 65, 96), 8),
                                           ((2, 17, 31, 64), 64), ((1, 3, 129, 640), 32), ((2, 6, 10, 2048), 2048), ((1, 7, 5, 2040), 3), ((1, 200, 190, 16), 2),
-                                          ((5, 61, 67, 72), 1), ((2, 300, 301, 8), 8), ((1, 90, 160, 256), 16), ((300, 4, 4, 32), 4)])
+                                          ((5, 61, 67, 72), 1), ((2, 300, 301, 8), 8), ((1, 90, 160, 256), 16), ((300, 4, 4, 32), 4), ((2, 36, 126, 600), 1), ((1, 20, 130, 2048), 2),
+                                          ((3, 50, 40, 1024), 4)])
 def test_shapes(hip, shape, groups, dtype):
     x, gamma, beta = make(shape, dtype)
     got = hip.group_norm(x, groups, gamma, beta, act=hip.ACT_RELU)

@@ -49,7 +49,7 @@ def check_codes(hip, x):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("rows,K", [(1, 1), (3, 5), (45, 512), (7, 1000), (64, 1024), (5, 1025), (130, 1960), (9, 2048), (3, 2056), (6, 4096), (2, 5001), (3, 8192), (2, 16384),
-                                    (2, 16392), (1, 20003), (1, 131072), (1000, 8), (3, 61), (66000, 16)])
+                                    (2, 16392), (1, 20003), (1, 131072), (1000, 8), (3, 61), (66000, 16), (700, 1023), (300, 4099), (9, 3), (33, 16390)])
 def test_codes(hip, rows, K, dtype):
     check_codes(hip, rand((rows, K), dtype, rows + K))
 
@@ -154,7 +154,7 @@ def test_large_products(hip, conv, M, K, N):
 
 
 @pytest.mark.parametrize("dtype,odt", [(torch.float16, torch.float16), (torch.float32, torch.float16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (1, 4097, 70), (2, 4096, 33), (1, 8192, 64), (3, 64, 64), (4, 4096, 70), (16, 1024, 40), (1, 16384, 70), (1, 16383, 64), (15, 1000, 33), (16, 1025, 64), (5, 7, 3), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32)])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (1, 4097, 70), (2, 4096, 33), (1, 8192, 64), (3, 64, 64), (4, 4096, 70), (16, 1024, 40), (1, 16384, 70), (1, 16383, 64), (15, 1000, 33), (16, 1025, 64), (5, 7, 3), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32), (900, 253, 787), (40, 1021, 35)])
 def test_layer_on_float_tokens(hip, conv, M, K, N, dtype, odt):
     layer, wq, ws, b = layer_of(conv, N, K, 5)
     x = rand((M, K), dtype, 6)

@@ -107,3 +107,27 @@ def test_masked_windows_are_a_batch_behind_their_pooled_tokens(hip, T, tind):
     pa.check(got, ref, bound)
     there = want[:, own.long()].permute(1, 0, 2, 3, 4).reshape(nW, T * 45, heads, 128)
     pa.check(there, ref, bound)
+
+
+def test_outputs_over_inputs_are_refused(hip):
+    from propainter_amd import conv
+    x = torch.randn(64, 256, device="cuda", dtype=torch.float16)
+    layer = conv.Int8Linear(torch.randn(128, 256), None)
+    with pytest.raises(ValueError, match="overlaps"):
+        layer(x, out=x)
+    with pytest.raises(ValueError, match="overlaps"):
+        layer(x[:1], out=x[:1, 64:])
+    both = torch.randn(64, 384, device="cuda", dtype=torch.float16)      # side by side in one buffer
+    want = layer(both[:, :256].clone())
+    layer(both[:, :256], out=both[:, 256:])
+    assert torch.equal(both[:, 256:], want)
+    with pytest.raises(ValueError, match="overlaps"):
+        layer(both[:, :256], out=both[:, 248:])
+    q = torch.randn(2, 3, 2, 64, device="cuda", dtype=torch.float16)
+    kv = torch.randn(2, 2, 5, 2, 64, device="cuda", dtype=torch.float16)
+    for out in (q, kv[0][:, :3]):
+        with pytest.raises(ValueError, match="overlaps"):
+            hip.shared_prefix_attention(q, None, None, kv[0], kv[1], out=out)
+    m = torch.randn(5, 6, 6, 16, device="cuda", dtype=torch.float16)
+    with pytest.raises(ValueError, match="overlaps"):
+        hip.group_norm(m[:4], 4, out=m[1:])
