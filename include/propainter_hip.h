@@ -456,8 +456,7 @@ int pp_group_norm(const void* in, int in_cstride, int in_choff, void* out, int o
                   int dtype, void* stream);
 
 /* 8-bit codes of token rows: scale[r] = max_k |x[r, k]| / 127 (fp32), q[r, k] = x[r, k] / scale[r] rounded to the nearest integer, ties to
- * even, of the real quotient.  x: rows of K elements of dtype, x_rstride elements apart (any alignment of dtype; 16-byte aligned rows
- * are read in 16-byte pieces).  q: int8 rows, q_rstride bytes apart; columns [K, pp_i8_row_bytes(K)) are written as zeros, q and q_rstride
+ * even, of the real quotient.  x: rows of K elements of dtype, x_rstride elements apart (any alignment of dtype).  q: int8 rows, q_rstride bytes apart; columns [K, pp_i8_row_bytes(K)) are written as zeros, q and q_rstride
  * multiples of 16.  A row of zeros has scale 0 and codes 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that a
  * product with it is NaN.  rows may be 0. */
 int pp_i8_row_bytes(int K);            /* K rounded up to a multiple of 64 (0 < K <= 131072), else PP_ERR_ARG */
@@ -468,7 +467,7 @@ int pp_quantize_tokens(const void* x, int64_t x_rstride, void* q, int64_t q_rstr
  * xq / xs: codes and scales as pp_quantize_tokens writes them (rows of pp_i8_row_bytes(K) bytes, zeros past K, q_rstride bytes apart,
  * 16-byte aligned).  weight: codes int8 [N, K] (rows wq_rstride bytes apart) laid out once by pp_linear_i8_pack into
  * pp_linear_i8_weight_bytes(N, K) bytes, 16-byte aligned; ws fp32 [N]; bias fp32 [N] or NULL.  out: rows of out_dtype (PP_F32 / PP_F16),
- * out_rstride elements apart; columns past N are left as they are.  act: any PP_ACT_*.  M may be 0. */
+ * out_rstride elements apart, not over the inputs; columns past N are left as they are.  act: any PP_ACT_*.  M may be 0. */
 int64_t pp_linear_i8_weight_bytes(int N, int K);
 int pp_linear_i8_pack(const void* wq, int64_t wq_rstride, void* weight, int N, int K, void* stream);
 int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void* weight, const float* ws, const float* bias, void* out,
@@ -486,7 +485,8 @@ int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const voi
  * their common pooled tokens (model/modules/sparse_transformer.py:205-262) are such a batch, and so are single tokens behind a common
  * prompt.  Query head h reads key head h / (Hq / Hkv).  Of the prefix the first prefix_lens[g] of P keys count, of the suffix the first
  * lens[b] of S (values are clamped to [0, P] / [0, S]; what lies behind them is never used, NaN included); with causal = 1 query i sees
- * suffix keys up to lens[b] - Lq + i (the queries are the last Lq tokens of the sequence).  A query without keys gives zeros.
+ * suffix keys up to lens[b] - Lq + i (the queries are the last Lq tokens of the sequence), and the values hidden from it have to be finite.  A
+ * query without keys gives zeros.  out may not overlap an input.
  * Strides in elements, multiples of 8 (fp16) / 4 (fp32), the last dimension (D) contiguous, buffers 16-byte aligned; token strides >= D. */
 typedef struct {
   int32_t dtype;                        /* PP_F16 / PP_F32: q, keys, values, out                   */

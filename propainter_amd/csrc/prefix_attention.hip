@@ -9,11 +9,20 @@
 // suffix).  Where a row's keys are split over several blocks, each leaves (max, sum, unnormalised output) in fp32 scratch and
 // pa_join_kernel joins them in a fixed order.
 //
-// pa_tile_kernel: 4 waves, key tiles in LDS (K swizzled, V skewed), the next tile's global loads in flight during the products.
-//   S^T = K Q^T and O^T += V^T P^T on 16x16 MFMA tiles: a lane holds scores of ONE query (column l & 15), so the row maximum takes two
-//   lane swaps, and its scores are the second product's operand as they are, keys relabelled.
-//   WK = false: a wave owns 16 QT rows and every key of a tile (many rows).  WK = true: the four waves share 16 QT rows and take a quarter
-//   of a tile's keys each, joined through LDS at the end (few rows: single tokens).
+// S^T = K Q^T and O^T += V^T P^T on 16x16 MFMA tiles: a lane holds scores of ONE query (column l & 15), so the row maximum takes two lane
+// swaps, and its scores are the second product's operand as they are, keys relabelled.  Maximum, sum and output stay in fp32 registers;
+// fp16 weights are rounded once, to the values' type.
+//
+// Forms (4 waves a block).  Many rows: a wave owns 16 QT rows and every key of a tile of 64 that lies in LDS (K and V swizzled, fp32 V
+// skewed), the next tile's loads in flight during the products.  Few rows (WK): the four waves share 16 QT rows and take different keys,
+// joined through LDS at the end; in fp16 every wave streams keys of its own (pa_stream_block).
+//   rows: 24 sequences x 765 queries, 4 heads of 128, 2430 shared + 1158 own keys, fp16: 181 us = 750 TFLOP/s.  Products alone would be 117 us at the rate
+//     of a large matrix product; the softmax' vector instructions take 190 of 407 thousand cycles a CU next to 130 of MFMA, and two blocks a
+//     CU overlap them in part.  LDS conflicts: none.  Two LDS tiles (one barrier a tile, one block a CU): 193.
+//   single tokens: 64 sequences, 8192 shared + up to 1024 own keys, 32 heads on 8 key heads of 128, fp16: 55 us for 171 MB; the two parts run in one launch
+//     (44 us: the suffixes out of memory next to the packed rows' products), 6 us of joining, the rest launches.
+//   fp32: 16 sequences x 4 queries, 16 heads on 2 key heads of 64, 4096 + up to 512 keys: 26 us, of which 6.6 are products at the fp32 matrix
+//     rate; few waves, so the latency of a tile's loads and dependent products, and the join's 6 us.
 #include "common.h"
 #include "attn_lanes.h"
 
