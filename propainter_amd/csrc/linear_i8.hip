@@ -661,8 +661,10 @@ static void launch_thin(const LinI8Params& p, hipStream_t st) {
   hipLaunchKernelGGL((lin_i8_thin_kernel<TO, MT, TPB>), dim3((unsigned)((p.N + 63) / 64 * (4 / TPB)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, p);
 }
 // Which form: measured at K = N = 4096 unless said otherwise (us).
-//   thin, few 128 x 128 tiles (at most 64: they would leave most CUs idle) or few tokens: 16 tokens x 1024 -> 16384 6.0 against 8.5 with tiles, 64 tokens 10.5 against 22.7 with tiles, 256 tokens 15.5 against 23.3,
-//   512 tokens 28.7 against 23.8
+//   thin, few 128 x 128 tiles (at most 64: they would leave most CUs idle) or few tokens: 16 tokens x 1024 -> 16384 6.0 against 8.5 with tiles,
+//   64 tokens 10.5 against 22.7, 256 tokens 15.5 against 23.3, 512 tokens 28.7 against 23.8; 1084 x 7352 -> 760 25.4 against 30.0 with 64 x 128
+//   64 x 128 tiles, at most 128 of 128 x 128 (one a CU): 512 tokens 20.5 against 26.3, 1500 x 1024 -> 1024 8.4 against 10.9, 2935 x 4207 -> 988
+//   (184 tiles) 29.6 against 28.8
 //   stream, K <= 512 and enough token tiles for every resident block: 110160 x 512 -> 1536 134 against 166, 10000 tokens 16.4 against 17.3,
 //   5000 x 512 -> 512 7.9 against 6.8
 //   256 x 256 tiles where K is long and they fill the chip twice: 8192^3 487 against 505 with 128 x 256; 4096^3 65 either way
@@ -680,6 +682,8 @@ static void launch_product(const LinI8Params& p, hipStream_t st) {
     else launch_stream<TO, 8>(p, st);
   } else if (p.ktiles >= 96 && t256 >= 512) {
     launch_tiles<TO, 256, 256, 2, 4, 4, 1>(p, st);
+  } else if (t128 <= 128) {
+    launch_tiles<TO, 64, 128, 2, 2, 4, 3>(p, st);
   } else if (t256w >= 256) {
     launch_tiles<TO, 128, 256, 2, 4, 3, 4>(p, st);
   } else {

@@ -127,7 +127,7 @@ def layer_of(conv, N, K, seed, bias=True):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 4096, 512), (2, 100, 30), (3, 1960, 512), (5, 512, 17), (16, 512, 1536), (17, 640, 100), (31, 65, 64), (32, 256, 257), (45, 512, 1536),
          (64, 1000, 65), (65, 128, 48), (100, 192, 1000), (127, 512, 130), (129, 320, 200), (200, 2048, 384), (256, 256, 256), (257, 300, 511), (333, 4100, 72), (513, 576, 640),
-         (1025, 64, 24), (2500, 200, 264), (300, 16384, 16), (20, 130, 9000), (1100, 1000, 1030)]
+         (1025, 64, 24), (2500, 200, 264), (3400, 330, 450), (900, 70, 2000), (70, 1000, 12000), (300, 16384, 16), (20, 130, 9000), (1100, 1000, 1030)]
 # weights kept in registers (K <= 256, K <= 512, odd channel blocks), 128 x 256 tiles, 256 x 256 tiles
 LARGE = [(49200, 200, 200), (17000, 500, 1000), (50000, 65, 70), (25001, 512, 520), (4200, 600, 2100), (8200, 1960, 770), (8100, 6200, 4100)]
 
