@@ -474,8 +474,8 @@ int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, const void*
                  int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* stream);
 
 /* pp_quantize_tokens and pp_linear_i8 in one call on float tokens x (rows of K elements of x_dtype, x_rstride elements apart).  work: device
- * scratch of pp_linear_i8_tokens_workspace_bytes(M, K) bytes, 16-byte aligned (0 for few tokens: one kernel does both). */
-int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int K);
+ * scratch of pp_linear_i8_tokens_workspace_bytes(M, N, K) bytes, 16-byte aligned (0 for small calls: one kernel does both). */
+int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int N, int K);
 int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const void* weight, const float* ws, const float* bias, void* out,
                         int64_t out_rstride, int64_t M, int N, int K, int act, float act_param, int out_dtype, void* work,
                         int64_t work_bytes, void* stream);

@@ -353,9 +353,9 @@ __device__ __forceinline__ void thin_product(const u32x4* w, int kt0, int kt1, i
 #endif
 }
 
-// adds the waves' sums and writes the block's outputs; xs_of(m) is the scale of token m
+// adds the waves' sums and writes the block's outputs, tokens m0 .. m_end - 1; xs_of(m) is the scale of token m
 template <typename TO, int MT, int TPB, typename F>
-__device__ __forceinline__ void thin_finish(const LinI8Params& p, i32x4* red, const i32x4 (&acc)[TPB][MT], int nb, int t0, long long m0, F xs_of) {
+__device__ __forceinline__ void thin_finish(const LinI8Params& p, i32x4* red, const i32x4 (&acc)[TPB][MT], int nb, int t0, long long m0, long long m_end, F xs_of) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int t = 0; t < TPB; ++t)
@@ -369,7 +369,7 @@ __device__ __forceinline__ void thin_finish(const LinI8Params& p, i32x4* red, co
     const int t = t0 + f / MT;
     const long long m = m0 + f % MT * 16 + (lane & 15);
     const int c = nb * 64 + (t >> 1) * 32 + (lane >> 4) * 8 + (t & 1) * 4;
-    if (m >= p.M) continue;
+    if (m >= m_end) continue;
     const float xs = xs_of(m);
     TO* o = reinterpret_cast<TO*>(p.out) + m * p.ors + c;
 #pragma unroll
@@ -400,23 +400,31 @@ __global__ __launch_bounds__(512) void lin_i8_thin_kernel(const LinI8Params p) {
     for (int j = 0; j < MT; ++j) acc[t][j] = i32x4{0, 0, 0, 0};
   thin_product<MT, TPB>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
                         [&](int kt, int j) { return *reinterpret_cast<const i32x4*>(xa[j] + (long long)kt * 64); });
-  thin_finish<TO, MT, TPB>(p, red, acc, nb, t0, m0, [&](long long m) { return p.xs[m]; });
+  thin_finish<TO, MT, TPB>(p, red, acc, nb, t0, m0, p.M, [&](long long m) { return p.xs[m]; });
 }
 
-// Few float tokens (at most 16, 2048 vectors of 8 in all): every block makes their codes itself, into LDS -- they come out of L2, and a launch and a
-// round trip of the codes are saved.  4096 -> 4096: one token 8.0 us against 7.0 for the product alone plus a launch for the codes, four
-// tokens 10.4 against 7.2 plus that launch.
+// Small calls on float tokens: a block takes up to 16 tokens (2048 vectors of 8 in all) and 16 channels and makes the tokens' codes itself, into LDS --
+// they come out of L2, and a launch and a round trip of the codes are saved.  Replayed / called (us): 45 x 512 -> 1536 5.7 / 9 against 6.5 / 14.4 with
+// two launches, 200 x 512 -> 512 6.6 / 9 against 7.4 / 14.6; with more blocks every one of them quantises too much: 400 x 512 -> 512 (800 blocks)
+// 9.3 against 7.6 replayed.  One token is always taken here.
 constexpr int I8_FUSE_VEC = 4;                     // vectors a thread
-inline bool i8_fused(int64_t M, int K) { return M <= 16 && M * ((K + 63) / 64 * 8) <= 512 * I8_FUSE_VEC; }
+constexpr int64_t I8_FUSE_BLOCKS = 512;            // two a CU
+inline int i8_fused_rows(int64_t M, int N, int K) {  // tokens a block (0: two launches)
+  int rows = 512 * I8_FUSE_VEC / ((K + 63) / 64 * 8);
+  if (rows > 16) rows = 16;
+  if (rows > M) rows = (int)M;
+  return rows > 0 && (M == 1 || (M + rows - 1) / rows * ((N + 63) / 64 * 4) <= I8_FUSE_BLOCKS) ? rows : 0;
+}
 template <typename T, typename TO>
-__global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, const FloatTokens<T> x) {
+__global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, const FloatTokens<T> x, const int rows) {
   __shared__ __attribute__((aligned(16))) i32x4 red[I8_KW * 64];
   __shared__ __attribute__((aligned(16))) int8_t codes[512 * I8_FUSE_VEC * 8 + 16 * 16];       // rows of K padded to 64, 16 bytes apart
   __shared__ unsigned rmax[16];
   __shared__ float xs[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nb = blockIdx.x >> 2, t0 = blockIdx.x & 3;
-  const int M = (int)p.M, Kp = p.ktiles * 64, vr = Kp >> 3, ld = Kp + 16;
+  const long long m0 = (long long)blockIdx.y * rows;
+  const int M = (int)min((long long)rows, p.M - m0), Kp = p.ktiles * 64, vr = Kp >> 3, ld = Kp + 16;
   if (threadIdx.x < 16) rmax[threadIdx.x] = 0;
   __syncthreads();
   Raw8<T> raw[I8_FUSE_VEC];
@@ -427,7 +435,7 @@ __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, 
     row[v] = r < M ? r : -1;
     raw[v].clear();
     if (row[v] >= 0 && c < x.K) {
-      const T* xr = x.x + (long long)r * x.xrs + c;
+      const T* xr = x.x + (m0 + r) * x.xrs + c;
       if (c + 8 <= x.K) {
         raw[v].load_any(xr);
       } else {
@@ -461,7 +469,7 @@ __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, 
   const int8_t* xa = codes + ((lane & 15) < M ? lane & 15 : 0) * ld + (lane >> 4) * 16;        // (columns past M repeat row 0 and are not stored)
   thin_product<1, 1>(w, (int)((long long)p.ktiles * wave / I8_KW), (int)((long long)p.ktiles * (wave + 1) / I8_KW), acc,
                      [&](int kt, int) { return *reinterpret_cast<const i32x4*>(xa + kt * 64); });
-  thin_finish<TO, 1, 1>(p, red, acc, nb, t0, 0, [&](long long m) { return xs[m]; });
+  thin_finish<TO, 1, 1>(p, red, acc, nb, t0, m0, m0 + M, [&](long long m) { return xs[m - m0]; });
 }
 
 // Tiles of BM tokens x BN channels, WM x WN waves of BM / WM tokens x BN / WN channels.  Both operands go from memory into LDS without
@@ -786,10 +794,10 @@ extern "C" int pp_linear_i8(const void* xq, int64_t q_rstride, const float* xs, 
   return launch_status("pp_linear_i8");
 }
 
-extern "C" int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int K) {
+extern "C" int64_t pp_linear_i8_tokens_workspace_bytes(int64_t M, int N, int K) {
   const int Kp = pp_i8_row_bytes(K);
-  if (Kp <= 0 || M < 0 || M > PP_I8_MAX_M) return PP_ERR_ARG;
-  return i8_fused(M, K) ? 0 : M * Kp + M * 4;
+  if (Kp <= 0 || N <= 0 || N > PP_I8_MAX_N || M < 0 || M > PP_I8_MAX_M) return PP_ERR_ARG;
+  return M == 0 || i8_fused_rows(M, N, K) ? 0 : M * Kp + M * 4;
 }
 
 extern "C" int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const void* weight, const float* ws, const float* bias, void* out,
@@ -802,7 +810,7 @@ extern "C" int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype
   const int esz = x_dtype == PP_F16 ? 2 : 4, Kp = pp_i8_row_bytes(K);
   PP_REQUIRE(x && x_rstride >= 0, PP_ERR_ARG, "pp_linear_i8_tokens: null tokens or row stride %lld", (long long)x_rstride);
   PP_REQUIRE((uintptr_t)x % esz == 0, PP_ERR_ALIGN, "pp_linear_i8_tokens: misaligned tokens");
-  const int64_t need = pp_linear_i8_tokens_workspace_bytes(M, K);
+  const int64_t need = pp_linear_i8_tokens_workspace_bytes(M, N, K);
   PP_REQUIRE(need == 0 || (work != nullptr && work_bytes >= need && (uintptr_t)work % 16 == 0), PP_ERR_WORKSPACE,
              "pp_linear_i8_tokens: needs %lld bytes of 16-byte aligned scratch, got %lld", (long long)need, (long long)work_bytes);
   int8_t* q = (int8_t*)work;
@@ -812,8 +820,10 @@ extern "C" int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype
     return pp_linear_i8(q, Kp, xs, weight, ws, bias, out, out_rstride, M, N, K, act, act_param, out_dtype, stream);
   }
   const LinI8Params p = lin_i8_params(nullptr, 0, nullptr, weight, ws, bias, out, out_rstride, M, N, K, act, act_param);
-  const dim3 grid((unsigned)((N + 63) / 64 * 4)), block(512);
-#define PP_TOKEN(T, TO) hipLaunchKernelGGL((lin_i8_token_kernel<T, TO>), grid, block, 0, (hipStream_t)stream, p, FloatTokens<T>{(const T*)x, (long long)x_rstride, K})
+  const int rows = i8_fused_rows(M, N, K);
+  const dim3 grid((unsigned)((N + 63) / 64 * 4), (unsigned)((M + rows - 1) / rows)), block(512);
+#define PP_TOKEN(T, TO) \
+  hipLaunchKernelGGL((lin_i8_token_kernel<T, TO>), grid, block, 0, (hipStream_t)stream, p, FloatTokens<T>{(const T*)x, (long long)x_rstride, K}, rows)
   if (x_dtype == PP_F16) { if (out_dtype == PP_F16) PP_TOKEN(_Float16, _Float16); else PP_TOKEN(_Float16, float); }
   else { if (out_dtype == PP_F16) PP_TOKEN(float, _Float16); else PP_TOKEN(float, float); }
 #undef PP_TOKEN

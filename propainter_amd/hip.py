@@ -79,7 +79,7 @@ _CTYPES = {"p": C.c_void_p, "i": C.c_int, "l": C.c_int64, "f": C.c_float}
 _TOKEN_OPS = {
     "pp_group_norm_workspace_floats": ("l", "iiiii"), "pp_group_norm": ("i", "piipiipppiiiiififip"),
     "pp_i8_row_bytes": ("i", "i"), "pp_quantize_tokens": ("i", "plplpliip"), "pp_linear_i8_weight_bytes": ("l", "ii"),
-    "pp_linear_i8_pack": ("i", "plpiip"), "pp_linear_i8": ("i", "plppppplliiifip"), "pp_linear_i8_tokens_workspace_bytes": ("l", "li"),
+    "pp_linear_i8_pack": ("i", "plpiip"), "pp_linear_i8": ("i", "plppppplliiifip"), "pp_linear_i8_tokens_workspace_bytes": ("l", "lii"),
     "pp_linear_i8_tokens": ("i", "plippppl" + "liiifipl" + "p"),
     "pp_shared_prefix_attention_workspace_bytes": ("l", "p"), "pp_shared_prefix_attention": ("i", "pp"),
 }
@@ -957,7 +957,7 @@ def linear_i8_tokens(x, weight, wscale, bias, N, act=ACT_NONE, act_param=0.0, ou
     stream = _raw_stream("linear_i8_tokens", x, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
     if M:
-        need = lib().pp_linear_i8_tokens_workspace_bytes(M, K)
+        need = lib().pp_linear_i8_tokens_workspace_bytes(M, N, K)
         work = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
         _launch("pp_linear_i8_tokens", "linear_i8", 2.0 * M * N * K, M * K * x.element_size() + weight.numel() + M * N * out.element_size(), (x, weight, wscale, bias),
                 (out, work), lib().pp_linear_i8_tokens, x.data_ptr(), rs, xcode, weight.data_ptr(), wscale.data_ptr(), _ptr(bias), out.data_ptr(), ors, M, N, K, act,

@@ -154,7 +154,8 @@ def test_large_products(hip, conv, M, K, N):
 
 
 @pytest.mark.parametrize("dtype,odt", [(torch.float16, torch.float16), (torch.float32, torch.float16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (1, 4097, 70), (2, 4096, 33), (1, 8192, 64), (3, 64, 64), (4, 4096, 70), (16, 1024, 40), (1, 16384, 70), (1, 16383, 64), (15, 1000, 33), (16, 1025, 64), (5, 7, 3), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32), (900, 253, 787), (40, 1021, 35)])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 100), (2, 1030, 512), (1, 4097, 70), (2, 4096, 33), (1, 8192, 64), (3, 64, 64), (4, 4096, 70), (16, 1024, 40), (1, 16384, 70), (1, 16383, 64), (15, 1000, 33), (16, 1025, 64), (5, 7, 3), (7, 4096, 192), (16, 100, 65), (45, 512, 1536), (700, 1960, 136), (1, 20000, 32), (900, 253, 787), (40, 1021, 35), (17, 512, 1536), (33, 2188, 70), (100, 64, 100), (23, 9000, 30),
+                                   (400, 300, 20), (16, 512, 17000), (1000, 65, 64), (9, 16384, 20)])
 def test_layer_on_float_tokens(hip, conv, M, K, N, dtype, odt):
     layer, wq, ws, b = layer_of(conv, N, K, 5)
     x = rand((M, K), dtype, 6)

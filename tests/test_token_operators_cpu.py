@@ -69,21 +69,21 @@ def test_linear_i8_refuses(L, kw, rc):
     assert lin(L, **kw) == rc
 
 
-def tokens(L, x=A, xrs=100, xdt=1, w=A, ws=A, out=A, ors=80, M=40, N=80, K=100, act=0, odt=1, work=A, wb=1 << 20):
+def tokens(L, x=A, xrs=100, xdt=1, w=A, ws=A, out=A, ors=80, M=4000, N=80, K=100, act=0, odt=1, work=A, wb=1 << 20):
     return L.pp_linear_i8_tokens(ptr(x), C.c_int64(xrs), C.c_int(xdt), ptr(w), ptr(ws), None, ptr(out), C.c_int64(ors), C.c_int64(M), C.c_int(N), C.c_int(K), C.c_int(act),
                                  C.c_float(0), C.c_int(odt), ptr(work), C.c_int64(wb), None)
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(x=0), ARG), (dict(w=0), ARG), (dict(ws=0), ARG), (dict(out=0), ARG), (dict(M=-1), ARG), (dict(N=0), ARG), (dict(K=0), ARG), (dict(act=9), ARG),
                                    (dict(xdt=2), DTYPE), (dict(odt=5), DTYPE), (dict(xrs=-4), ARG), (dict(x=A + 1), ALIGN), (dict(w=A + 8), ALIGN), (dict(ors=79), ARG), (dict(work=0), WORK),
-                                   (dict(wb=40 * 128 + 159), WORK), (dict(work=A + 4), WORK), (dict(M=0), 0)])
+                                   (dict(wb=4000 * 132 - 1), WORK), (dict(work=A + 4), WORK), (dict(M=0), 0)])
 def test_linear_i8_tokens_refuses(L, kw, rc):
     assert tokens(L, **kw) == rc
 
 
 def test_linear_i8_tokens_workspace(L):
-    f = lambda m, k: L.pp_linear_i8_tokens_workspace_bytes(C.c_int64(m), C.c_int(k))  # noqa: E731
-    assert f(0, 64) == 0 and f(40, 100) == 40 * 128 + 160 and f(-1, 64) == ARG and f(1, 0) == ARG and f(1000, 131072) == 1000 * 131076
+    f = lambda m, k, n=80: L.pp_linear_i8_tokens_workspace_bytes(C.c_int64(m), C.c_int(n), C.c_int(k))  # noqa: E731
+    assert f(0, 64) == 0 and f(4000, 100) == 4000 * 132 and f(40, 100) == 0 and f(40, 100, 50000) == 40 * 132 and f(1, 100, 0) == ARG and f(1, 100, 4194241) == ARG and f(-1, 64) == ARG and f(1, 0) == ARG and f(1000, 131072) == 1000 * 131076
 
 
 def test_linear_i8_pack_refuses(L):
