@@ -913,7 +913,7 @@ def linear_i8_pack(wq, K=None):
     return w
 
 
-def _linear_i8_out(who, weight, wscale, bias, N, K, M, dtype, out, device):
+def _linear_i8_out(who, weight, wscale, bias, N, K, M, dtype, out, device, inputs):
     assert wscale.dtype == torch.float32 and wscale.is_contiguous() and wscale.shape == (N,)
     assert bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.shape == (N,))
     assert weight.dtype == torch.int8 and weight.is_contiguous() and weight.numel() == _linear_i8_bytes(N, K)
@@ -921,6 +921,7 @@ def _linear_i8_out(who, weight, wscale, bias, N, K, M, dtype, out, device):
         return torch.empty((M, N), dtype=dtype, device=device), N
     if out.dim() != 2 or out.shape[0] != M or out.shape[1] < N or (M and (out.stride(1) != 1 or (M > 1 and out.stride(0) < N))):
         raise ValueError(f"{who}: out must be [{M}, >= {N}] with contiguous rows")
+    _refuse_overlap(who, out[:, :N], *inputs, weight, wscale, bias)
     return out, max(out.stride(0), N)
 
 
@@ -934,9 +935,7 @@ def linear_i8(q, scale, weight, wscale, bias, N, K, act=ACT_NONE, act_param=0.0,
         raise ValueError(f"linear_i8: codes must be int8 [M, {Kp}] as quantize_tokens returns them, got {q.dtype} {tuple(q.shape)}")
     if scale.dtype != torch.float32 or scale.shape != (M,) or not scale.is_contiguous():
         raise ValueError(f"linear_i8: scales must be float32 [{M}]")
-    if out is not None:
-        _refuse_overlap("linear_i8", out[:, :N], q, scale, weight, wscale, bias)
-    out, ors = _linear_i8_out("linear_i8", weight, wscale, bias, N, K, M, out_dtype, out, q.device)
+    out, ors = _linear_i8_out("linear_i8", weight, wscale, bias, N, K, M, out_dtype, out, q.device, (q, scale))
     stream = _raw_stream("linear_i8", q, scale, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
     if M:
@@ -951,9 +950,7 @@ def linear_i8_tokens(x, weight, wscale, bias, N, act=ACT_NONE, act_param=0.0, ou
     require_gpu(x, "linear_i8_tokens")
     M, K, rs = _token_rows("linear_i8_tokens", x)
     xcode, Kp = dtype_code(x.dtype), i8_row_bytes(K)
-    if out is not None:
-        _refuse_overlap("linear_i8_tokens", out[:, :N], x, weight, wscale, bias)
-    out, ors = _linear_i8_out("linear_i8_tokens", weight, wscale, bias, N, K, M, out_dtype or x.dtype, out, x.device)
+    out, ors = _linear_i8_out("linear_i8_tokens", weight, wscale, bias, N, K, M, out_dtype or x.dtype, out, x.device, (x,))
     stream = _raw_stream("linear_i8_tokens", x, weight, wscale, bias, out)
     code = dtype_code(out.dtype)
     if M:

@@ -123,6 +123,9 @@ def test_outputs_over_inputs_are_refused(hip):
     assert torch.equal(both[:, 256:], want)
     with pytest.raises(ValueError, match="overlaps"):
         layer(both[:, :256], out=both[:, 248:])
+    for bad in (torch.empty(64, device="cuda", dtype=torch.float16), torch.empty(63, 128, device="cuda", dtype=torch.float16)):
+        with pytest.raises(ValueError, match="out must be"):
+            layer(x, out=bad)
     q = torch.randn(2, 3, 2, 64, device="cuda", dtype=torch.float16)
     kv = torch.randn(2, 2, 5, 2, 64, device="cuda", dtype=torch.float16)
     for out in (q, kv[0][:, :3]):
