@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256, 2) void conv_ast_kernel(const ConvParams p) {
     }
     if (!prewaited) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     prewaited = false;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave's fragment reads of stage buf^1 are back
     __builtin_amdgcn_s_barrier();                     // stage `buf` landed for all waves; stage buf^1 is free
     {
       int nc = chunk, ns = step + 1;

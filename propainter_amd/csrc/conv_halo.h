@@ -323,6 +323,10 @@ __global__ __launch_bounds__(TH * TW * 128 / WMT, WMT == 32 ? 4 : HALO_MIN_WAVES
         PP_MFMA_PRIO_END();
       }
       }
+      // The step's fragment reads are back before the wave arrives at the next barrier (PRIVB: before its own next request): past it, any wave's DMA
+      // writes the stage they come from.  The compiler alone does not see to that: it moves products, and the waits for their operands with them, past
+      // the barrier, and a read that is held up by a neighbouring block's LDS traffic then returned the NEXT step's weights.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if constexpr (PROF) { asm volatile("s_nop 0" ::: "memory"); pf_comp += __builtin_readcyclecounter() - pf_a; }
       ++ks;
       par ^= 1;
