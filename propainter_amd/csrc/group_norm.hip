@@ -9,6 +9,7 @@
 // those three passes.
 #include "common.h"
 #include "attn_lanes.h"
+#include <type_traits>
 
 namespace pp {
 
@@ -50,44 +51,80 @@ __device__ __forceinline__ void join_parts(int per, int ng, int s0, float& cnt, 
   __syncthreads();
 }
 
-// 256 threads: column = 8 channels, the rest of the block walks the pixels of one slice.  Sums are taken relative to the slice's first
-// pixel (per channel), so that they hold deviations and not magnitudes.
+// 256 threads: column = 8 channels, the rest of the block walks the pixels of one slice, GN_U at a time: those are in registers, so their mean and
+// squared deviations are taken in two passes, and joined to what the thread has.  Values are taken relative to the slice's first pixel (per
+// channel), so that means hold deviations and not magnitudes; it may itself lie far from the rest (a border of zeros): nothing is subtracted
+// from sums of squares.
+constexpr int GN_U = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   __shared__ float s1[256 * 8], s2[256 * 8], parts[3][256];
   const int c8 = p.C >> 3, rows = 256 / c8;
   const int t = threadIdx.x, col = t % c8, pr = t / c8;
-  const bool on = pr < rows;
   const int slice = blockIdx.x, n = blockIdx.y;
   const int p0 = slice * p.ppslice;
   const int np = min(p.ppslice, p.HW - p0);
+  const int last = pr < rows ? np : 0;               // threads past the last whole row of columns have no pixels
   const T* x = reinterpret_cast<const T*>(p.in) + ((long long)n * p.HW + p0) * p.in_cs + p.in_co + col * 8;
-  float shift[8], a[8], b[8];
+  float shift[8], m[8], M2[8], cnt = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-  if (on) {
-    load8<T>(x, shift);
-    for (int q = pr; q < np; q += rows) {
-      float v[8];
-      load8<T>(x + (long long)q * p.in_cs, v);
+  for (int i = 0; i < 8; ++i) m[i] = M2[i] = 0.f;
+  if (last > 0) load8<T>(x, shift);
+  // pixels q, q + rows, ..: all GN_U of them, or (FULL false) those below last
+  auto batch = [&](int q, auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    float v[GN_U][8];
+    const float nb = FULL ? (float)GN_U : (float)((last - q + rows - 1) / rows);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[i] - shift[i];
-        a[i] += d;
-        b[i] = fmaf(d, d, b[i]);
-      }
+    for (int u = 0; u < GN_U; ++u)
+      if (FULL || q + u * rows < last) load8<T>(x + (long long)(q + u * rows) * p.in_cs, v[u]);
+    const float nt = cnt + nb, f = nb / nt, w = cnt * f, rb = 1.f / nb;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float sum = 0.f, dev = 0.f;
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u)
+        if (FULL || q + u * rows < last) {
+          v[u][i] -= shift[i];
+          sum += v[u][i];
+        }
+      const float mb = sum * rb;
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u)
+        if (FULL || q + u * rows < last) {
+          const float d = v[u][i] - mb;
+          dev = fmaf(d, d, dev);
+        }
+      const float d = mb - m[i];
+      m[i] = fmaf(d, f, m[i]);
+      M2[i] = M2[i] + dev + d * w * d;
     }
-  }
+    cnt = nt;
+  };
+  int q = pr;
+  for (; q + (GN_U - 1) * rows < last; q += GN_U * rows) batch(q, std::true_type{});
+  if (q < last) batch(q, std::false_type{});
+  parts[0][t] = cnt;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { s1[t * 8 + i] = a[i]; s2[t * 8 + i] = b[i]; }
+  for (int i = 0; i < 8; ++i) { s1[t * 8 + i] = m[i]; s2[t * 8 + i] = M2[i]; }
   for (int h = rows; h > 1;) {                       // rows of the block, halved
     const int half = (h + 1) >> 1;
     __syncthreads();
     if (pr < h - half) {
+      const int o = t + half * c8;
+      const float nb = parts[0][o];
+      if (nb > 0.f) {                                // (a row without pixels lies behind those with pixels)
+        const float nt = cnt + nb, f = nb / nt, w = cnt * f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s1[t * 8 + i] += s1[(t + half * c8) * 8 + i];
-        s2[t * 8 + i] += s2[(t + half * c8) * 8 + i];
+        for (int i = 0; i < 8; ++i) {
+          const float d = s1[o * 8 + i] - m[i];
+          m[i] = fmaf(d, f, m[i]);
+          M2[i] = M2[i] + s2[o * 8 + i] + d * w * d;
+          s1[t * 8 + i] = m[i];
+          s2[t * 8 + i] = M2[i];
+        }
+        cnt = nt;
+        parts[0][t] = nt;
       }
     }
     h = half;
@@ -95,23 +132,19 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   __syncthreads();
   // per channel (mean, M2), then the channels of each group
   const T* x0 = reinterpret_cast<const T*>(p.in) + ((long long)n * p.HW + p0) * p.in_cs + p.in_co;
-  for (int c = t; c < p.C; c += 256) {
-    const float m = s1[c] / (float)np;
-    s2[c] = fmaxf(s2[c] - s1[c] * m, s2[c] - s2[c]);      // >= 0; NaN stays NaN
-    s1[c] = to_f32(x0[c]) + m;
-  }
+  for (int c = t; c < p.C; c += 256) s1[c] += to_f32(x0[c]);
   __syncthreads();
   const int per = p.groups < 256 ? 256 / p.groups : 1;   // threads that share one group's channels
   for (int g0 = 0; g0 < p.groups; g0 += 256) {
     const int ng = min(256, p.groups - g0), g = g0 + t % ng, s0 = t / ng;
-    float cnt = 0.f, m = 0.f, M2 = 0.f;
+    float gn = 0.f, gm = 0.f, gM2 = 0.f;
     if (s0 < per)
-      for (int c = s0; c < p.cg; c += per) chan_merge(cnt, m, M2, (float)np, s1[g * p.cg + c], s2[g * p.cg + c]);
-    join_parts(per, ng, s0, cnt, m, M2, parts);
+      for (int c = s0; c < p.cg; c += per) chan_merge(gn, gm, gM2, (float)np, s1[g * p.cg + c], s2[g * p.cg + c]);
+    join_parts(per, ng, s0, gn, gm, gM2, parts);
     if (s0 == 0) {
       float* o = p.part + (((long long)n * p.slices + slice) * p.groups + g) * 2;
-      o[0] = m;
-      o[1] = M2;
+      o[0] = gm;
+      o[1] = gM2;
     }
   }
 }
@@ -271,7 +304,7 @@ static int gn_group_block(int64_t HW, int C, int groups) {      // threads, 0: i
 }
 
 static void gn_split(int N, int HW, int C, int* slices, int* ppslice) {
-  // enough blocks to fill the chip, but no slice under 64 vectors a column set (the joins would cost more than the pixels)
+  // enough blocks to fill the chip, but no slice under 4 pixels a thread (the joins would cost more than the pixels)
   const int rows = 256 / (C / 8) > 0 ? 256 / (C / 8) : 1;
   int want = 1024 / N;
   if (want < 1) want = 1;
