@@ -65,6 +65,11 @@ __device__ __forceinline__ PaRow pa_row(int Lq, int rep, int nper, int space, in
 
 constexpr float PA_NONE = -3.4028235e38f;   // running maximum before the first key: finite, so that masked scores (-inf) weigh 0
 
+// fp16 weights are lifted: 2^15 for the maximum, so that one of 2^-29 of it still has its 11 bits and one of 2^-39 is not lost (unlifted 2^-14 and
+// 2^-24: behind a million keys the tail of a softmax would be).  The running maximum is kept less the lift; sums and outputs carry the factor, which
+// the last division takes out.
+template <typename T> constexpr float pa_lift() { return sizeof(T) == 2 ? 15.f : 0.f; }
+
 __device__ __forceinline__ int clamp_len(const int* lens, int i, int most) {
   const int n = lens != nullptr ? lens[i] : most;
   return n < 0 ? 0 : (n > most ? most : n);
@@ -354,7 +359,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
 #pragma unroll
         for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
       tmax = rows_max(tmax);
-      const float m_new = fmaxf(m_run[qt], tmax * p.sc2);
+      const float m_new = fmaxf(m_run[qt], fmaf(tmax, p.sc2, -pa_lift<T>()));
       const bool moved = m_new > m_run[qt];
       float psum = 0.f;
 #pragma unroll
@@ -590,7 +595,7 @@ __device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart&
 #pragma unroll
         for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
       tmax = rows_max(tmax);
-      const float m_new = fmaxf(m_run[qt], tmax * p.sc2);
+      const float m_new = fmaxf(m_run[qt], fmaf(tmax, p.sc2, -pa_lift<T>()));
       const bool moved = m_new > m_run[qt];
       float psum = 0.f;
 #pragma unroll
