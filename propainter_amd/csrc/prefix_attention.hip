@@ -65,10 +65,49 @@ __device__ __forceinline__ PaRow pa_row(int Lq, int rep, int nper, int space, in
 
 constexpr float PA_NONE = -3.4028235e38f;   // running maximum before the first key: finite, so that masked scores (-inf) weigh 0
 
-// fp16 weights are lifted: 2^15 for the maximum, so that one of 2^-29 of it still has its 11 bits and one of 2^-39 is not lost (unlifted 2^-14 and
-// 2^-24: behind a million keys the tail of a softmax would be).  The running maximum is kept less the lift; sums and outputs carry the factor, which
-// the last division takes out.
+// A weight is exp2((s - m) sc2 + lift) for the score s and the row's maximum m, both as the products left them.  fp16 weights are lifted: 2^15 for the
+// maximum, so that one of 2^-29 of it still has its 11 bits and one of 2^-39 is not lost (unlifted 2^-14 and 2^-24: behind a million keys the tail of a
+// softmax would be).  Sums and outputs carry the same factor, which the last division takes out.
 template <typename T> constexpr float pa_lift() { return sizeof(T) == 2 ? 15.f : 0.f; }
+// s sc2 + c with c = lift - m sc2 is one operation a score; c's own rounding scales all weights of the row alike.  Past 2^20 that factor could
+// leave the weights' range, so there the scores' differences are taken first (by the whole wave; such scores are that uncertain anyway).
+constexpr float PA_BIG = 1048576.f;
+template <int QT> struct PaRows { float m[QT], l[QT]; };      // running maximum, sum of the weights of this lane's keys
+template <int QT, int DT>
+__device__ __forceinline__ void pa_rows_start(PaRows<QT>& w, f32x4 (&oacc)[QT][DT]) {
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    w.m[qt] = PA_NONE;
+    w.l[qt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+// c of a row's new maximum
+template <typename T, int N>
+__device__ __forceinline__ float pa_base(const float m_new, const float sc2, f32x4 (&s)[N]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float c = fminf(fmaf(-m_new, sc2, pa_lift<T>()), -PA_NONE);
+  if (__builtin_amdgcn_ballot_w64(fabsf(c) > PA_BIG && m_new > PA_NONE) == 0ull) return c;
+#pragma unroll
+  for (int kt = 0; kt < N; ++kt) s[kt] -= m_new;
+#endif
+  return pa_lift<T>();
+}
+// adds a tile's weights to a row's sum; what is summed so far is scaled to the new maximum
+template <int QT, int DT>
+__device__ __forceinline__ void pa_rows_add(PaRows<QT>& w, f32x4 (&oacc)[QT][DT], const int qt, const float m_new, const float psum, const float sc2) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if (__builtin_amdgcn_ballot_w64(m_new > w.m[qt]) != 0ull) {
+    const float alpha = __builtin_amdgcn_exp2f((w.m[qt] - m_new) * sc2);
+    w.l[qt] *= alpha;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) oacc[qt][d] *= alpha;
+  }
+  w.m[qt] = m_new;
+  w.l[qt] += psum;
+#endif
+}
 
 __device__ __forceinline__ int clamp_len(const int* lens, int i, int most) {
   const int n = lens != nullptr ? lens[i] : most;
@@ -131,8 +170,8 @@ __device__ __forceinline__ PaItem pa_item(const PaParams& p, const PaPart& pt, c
 
 // The four waves of a block hold the same 16 QT rows for different keys: joined through LDS, then written out (or left in the scratch)
 template <typename T, int D, int QT>
-__device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& pt, char* lds, float* wave_ml, const f32x4 (&oacc)[QT][D / 16], const float (&m_run)[QT],
-                                              const float (&l_run)[QT], const long long (&rowid)[QT], char* const (&optr)[QT], const bool whole, const int split,
+__device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& pt, char* lds, float* wave_ml, const f32x4 (&oacc)[QT][D / 16], const PaRows<QT>& w,
+                                              const long long (&rowid)[QT], char* const (&optr)[QT], const bool whole, const int split,
                                               const bool any) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool F16 = sizeof(T) == 2;
@@ -144,9 +183,9 @@ __device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& p
   float l[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    l[qt] = rows_sum(l_run[qt]);
+    l[qt] = rows_sum(w.l[qt]);
     if (lg == 0) {
-      wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2] = m_run[qt];
+      wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2] = w.m[qt];
       wave_ml[(wave * 16 * QT + qt * 16 + lc) * 2 + 1] = l[qt];
     }
   }
@@ -159,8 +198,8 @@ __device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& p
     mj[qt] = fmaxf(fmaxf(e[0], e[W]), fmaxf(e[2 * W], e[3 * W]));
     lj[qt] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) lj[qt] += e[w * W + 1] * __builtin_amdgcn_exp2f(e[w * W] - mj[qt]);
-    const float f = __builtin_amdgcn_exp2f(m_run[qt] - mj[qt]);
+    for (int i = 0; i < 4; ++i) lj[qt] += e[i * W + 1] * __builtin_amdgcn_exp2f((e[i * W] - mj[qt]) * p.sc2);
+    const float f = __builtin_amdgcn_exp2f((w.m[qt] - mj[qt]) * p.sc2);
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 * QT + qt * 16 + lc) * JLD + d * 16 + lg * 4) = oacc[qt][d] * f;
   }
@@ -179,7 +218,7 @@ __device__ __forceinline__ void pa_join_waves(const PaParams& p, const PaPart& p
       const int pos = wave * (D / 4) + c * 16 + lg * 4;
       f32x4 v = *reinterpret_cast<const f32x4*>(e + pos);
 #pragma unroll
-      for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(e + w * W + pos);
+      for (int i = 1; i < 4; ++i) v += *reinterpret_cast<const f32x4*>(e + i * W + pos);
       if (!whole) {
         if (any) *reinterpret_cast<f32x4*>(p.part_o + at * D + pos) = v;
       } else if constexpr (F16) {
@@ -248,14 +287,8 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
   }
 
   f32x4 oacc[QT][DT];
-  float m_run[QT], l_run[QT];
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    m_run[qt] = PA_NONE;
-    l_run[qt] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  PaRows<QT> run;
+  pa_rows_start(run, oacc);
 
   // ---- staging: a tile's valid keys lie inside the buffer descriptor built for it, the rest (token strides are at least D) comes back as zeros,
   // so that nothing behind a length is used; 64-bit base per tile, 32-bit offsets inside it
@@ -359,26 +392,18 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
 #pragma unroll
         for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
       tmax = rows_max(tmax);
-      const float m_new = fmaxf(m_run[qt], fmaf(tmax, p.sc2, -pa_lift<T>()));
-      const bool moved = m_new > m_run[qt];
+      const float m_new = fmaxf(run.m[qt], tmax), base = pa_base<T>(m_new, p.sc2, sacc[qt]);
       float psum = 0.f;
 #pragma unroll
       for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, -m_new));
+          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, base));
           psum += e;
           if constexpr (C::F16) pfr[qt][kt >> 1][(kt & 1) * 4 + r] = (_Float16)e;    // weights in the values' type: the product's operand
           else sacc[qt][kt][r] = e;
         }
-      if (__builtin_amdgcn_ballot_w64(moved) != 0ull) {
-        const float alpha = __builtin_amdgcn_exp2f(m_run[qt] - m_new);
-        l_run[qt] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) oacc[qt][d] *= alpha;
-      }
-      m_run[qt] = m_new;
-      l_run[qt] += psum;                           // this lane's keys; the four lane groups are summed at the end
+      pa_rows_add(run, oacc, qt, m_new, psum, p.sc2);      // (this lane's keys; the four lane groups are summed at the end)
     }
     // ---- O^T += V^T P^T
     if constexpr (C::F16) {
@@ -424,11 +449,11 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
   if constexpr (!WK) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const float l = rows_sum(l_run[qt]);
+      const float l = rows_sum(run.l[qt]);
       if (rowid[qt] < 0) continue;
       if (!whole) {
         const long long at = (pt.slot0 + split) * p.prows + rowid[qt];
-        if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_run[qt], l);
+        if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(run.m[qt], l);
         if (t0 < t1) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + d * 16 + lg * 4) = oacc[qt][d];
@@ -451,7 +476,7 @@ __device__ __forceinline__ void pa_block(const PaParams& p, const PaPart& pt, co
       }
     }
   } else {
-    pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, m_run, l_run, rowid, optr, whole, split, t0 < t1);
+    pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, run, rowid, optr, whole, split, t0 < t1);
   }
 #endif
 }
@@ -494,7 +519,8 @@ __device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart&
   int vis[QT];
   char* optr[QT];
   f32x4 oacc[QT][DT];
-  float m_run[QT], l_run[QT];
+  PaRows<QT> run;
+  pa_rows_start(run, oacc);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int rl = qt * 16 + lc, r = row0 + rl;
@@ -510,10 +536,6 @@ __device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart&
       if (p.qsign != 1.f) f *= (T)p.qsign;
       qf[qt][s] = f;
     }
-    m_run[qt] = PA_NONE;
-    l_run[qt] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) oacc[qt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   u32x4 kf[C::DEPTH][2][STEPS], vr[C::DEPTH][VL];
@@ -595,25 +617,17 @@ __device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart&
 #pragma unroll
         for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sacc[qt][kt][r]);
       tmax = rows_max(tmax);
-      const float m_new = fmaxf(m_run[qt], fmaf(tmax, p.sc2, -pa_lift<T>()));
-      const bool moved = m_new > m_run[qt];
+      const float m_new = fmaxf(run.m[qt], tmax), base = pa_base<T>(m_new, p.sc2, sacc[qt]);
       float psum = 0.f;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, -m_new));
+          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[qt][kt][r], p.sc2, base));
           psum += e;
           pfr[qt][kt * 4 + r] = (_Float16)e;             // weights in the values' type: the product's operand
         }
-      if (__builtin_amdgcn_ballot_w64(moved) != 0ull) {
-        const float alpha = __builtin_amdgcn_exp2f(m_run[qt] - m_new);
-        l_run[qt] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) oacc[qt][d] *= alpha;
-      }
-      m_run[qt] = m_new;
-      l_run[qt] += psum;
+      pa_rows_add(run, oacc, qt, m_new, psum, p.sc2);
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -629,7 +643,7 @@ __device__ __forceinline__ void pa_stream_block(const PaParams& p, const PaPart&
     if constexpr (C::DEPTH == 2) chunk(t + 4, 1);         // (a chunk past the last one has no keys)
   }
   __syncthreads();                                         // every wave is done with its V rows: the join takes their place
-  pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, m_run, l_run, rowid, optr, whole, it.split, t0 < t1);
+  pa_join_waves<T, D, QT>(p, pt, lds, wave_ml, oacc, run, rowid, optr, whole, it.split, t0 < t1);
 #endif
 }
 
@@ -685,7 +699,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p, const in
   float mj = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mj = fmaxf(mj, __shfl_xor(mj, o));
-  const float wt = l != 0.f ? __builtin_amdgcn_exp2f(m - mj) : 0.f;
+  const float wt = l != 0.f ? __builtin_amdgcn_exp2f((m - mj) * p.sc2) : 0.f;
   float total = l != 0.f ? l * wt : 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);

@@ -1,7 +1,10 @@
-"""hip.shared_prefix_attention where weights far below the largest one count because they are many.
+"""hip.shared_prefix_attention where the softmax' range is wide: weights far below the largest one that count because they are many, and scores
+whose fp32 neighbours lie far apart.
 
-Bound: fp16 weights are held to 2^-11 of themselves and 2^-39 of the largest one (scores are exact here: one channel, small integers);
-n + 64 additions in fp32."""
+First bound: fp16 weights are held to 2^-11 of themselves and 2^-39 of the largest one (scores are exact here: one channel, small integers);
+n + 64 additions in fp32.  Second: products of powers of two are exact, keys of the same score weigh the same and a key behind by more than 200
+weighs nothing, so the output is a mean of at most n values: n 2^-24 of the mean size.  fp16 weights are rounded once as operands and not in their
+sum (sum round(w) v / sum w: at most 2^-11 of the mean size more; below 2^20 a score leaves the weights' common factor no power of two)."""
 import math
 
 import pytest
@@ -41,3 +44,36 @@ def test_many_small_weights_count(hip, B, Lq, Hq, Hkv, D, n, S, gap, dtype):
         rel = (n + 64 + gap) * 2.0 ** -24 + (2.0 ** -11 + 2.0 ** -39 * 2.0 ** (gap + 0.5) if dtype == torch.float16 else 0)
         lim = want * rel + want * torch.finfo(dtype).eps / 2 + 2.0 ** -25
         assert (got - want).abs().max().item() <= lim, ((got - want).abs().max().item(), want, lim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("size", [2.0 ** 11, -(2.0 ** 11), 2.0 ** 15, -(2.0 ** 15), 2.0 ** 60, -(2.0 ** 60), 2.0 ** 63, -(2.0 ** 63)])
+@pytest.mark.parametrize("B,Lq,Hq,Hkv,D,P,S", [(1, 1, 1, 1, 64, 0, 64), (3, 1, 4, 2, 128, 500, 12), (2, 90, 2, 2, 64, 200, 56), (64, 1, 8, 1, 128, 4000, 96), (2, 40, 4, 4, 128, 0, 128)])
+def test_scores_far_from_zero(hip, B, Lq, Hq, Hkv, D, P, S, size, dtype):
+    if dtype == torch.float16 and abs(size) > 2 ** 15:
+        pytest.skip("past fp16")
+    n = P + S
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, Hkv, D, generator=g, device="cuda").to(dtype)  # noqa: E731
+    q = torch.zeros(B, Lq, Hq, D, device="cuda", dtype=dtype)
+    q[..., 0] = abs(size)
+    k = lambda *s: torch.zeros(*s, Hkv, D, device="cuda", dtype=dtype)  # noqa: E731
+    pk, pv, ks, vs = (k(1, P), r(1, P), k(B, S), r(B, S)) if P else (None, None, k(B, S), r(B, S))
+    for t in (pk, ks):
+        if t is not None:
+            t[..., 0] = size
+    # every key the same score: the mean of all values
+    got = hip.shared_prefix_attention(q, pk, pv, ks, vs).double()
+    rep = Hq // Hkv
+    mean = lambda v: v.double().repeat_interleave(rep, 2)  # noqa: E731
+    every = mean(vs) if P == 0 else torch.cat([mean(pv).expand(B, -1, -1, -1), mean(vs)], 1)
+    lim = every.abs().mean(1, keepdim=True) * ((n + 64) * 2.0 ** -24 + (2.0 ** -11 if dtype == torch.float16 else 0)) + every.mean(1, keepdim=True).abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25
+    assert ((got - every.mean(1, keepdim=True)).abs() <= lim).all()
+    # four of them lead by a last place of the keys' type: the mean of those
+    lead = [0, S // 4, S // 2, S - 1]
+    ks[:, lead, :, 0] = size * (1 + torch.finfo(dtype).eps) if size > 0 else size * (1 - torch.finfo(dtype).eps / 2)
+    if abs(size) ** 2 * D ** -0.5 * torch.finfo(dtype).eps / 2 > 200:
+        got = hip.shared_prefix_attention(q, pk, pv, ks, vs).double()
+        four = mean(vs[:, lead]).mean(1, keepdim=True)
+        lim = mean(vs[:, lead]).abs().mean(1, keepdim=True) * (80 * 2.0 ** -24 + (2.0 ** -11 if dtype == torch.float16 else 0)) + four.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25
+        assert ((got - four).abs() <= lim).all()
