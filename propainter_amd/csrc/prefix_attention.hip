@@ -678,53 +678,53 @@ __global__ __launch_bounds__(256, (pa_waves<T, D, (QT0 > QT1 ? QT0 : QT1)>())) v
 template <typename T, int D>
 __global__ __launch_bounds__(256) void pa_join_kernel(const PaParams p, const int per) {
   const int lane = threadIdx.x & 63;
-  const long long row = blockIdx.x * 4ll + (threadIdx.x >> 6);
-  if (row >= p.prows) return;
   const PaPart& pt = p.part[0];
-  PaRow w;
-  if (pt.by_row) {
-    w = {(int)(row / p.Hq / p.Lq), (int)(row / p.Hq % p.Lq), (int)(row % p.Hq)};
-  } else {
-    const int item = pt.whole + (int)(row / per), rb = item % pt.rowblocks, r = rb * per + (int)(row % per);
-    if (r >= pt.rows) return;
-    w = pa_row(p.Lq, p.rep, pt.nper, item / pt.rowblocks / p.Hkv, item / pt.rowblocks % p.Hkv, r);
-  }
-  constexpr int E = D / 64, U = 8;
-  float m = PA_NONE, l = 0.f;                      // slots <= 64: one a lane
-  if (lane < p.slots) {
-    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + (lane * p.prows + row) * 2);
-    m = e.x;
-    l = e.y;
-  }
-  float mj = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mj = fmaxf(mj, __shfl_xor(mj, o));
-  const float wt = l != 0.f ? __builtin_amdgcn_exp2f((m - mj) * p.sc2) : 0.f;
-  float total = l != 0.f ? l * wt : 0.f;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  float acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  const float* src = p.part_o + row * D + lane * E;
-  for (int s0 = 0; s0 < p.slots; s0 += U) {
-    float v[U][E];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[u][e] = src[(long long)min(s0 + u, p.slots - 1) * p.prows * D + e];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int sl = min(s0 + u, 63);
-      const float ls = __shfl(l, sl), ws = __shfl(wt, sl);       // (lanes past the last slot: sum 0; a NaN sum is not 0 and stays)
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = s0 + u < p.slots && ls != 0.f ? fmaf(ws, v[u][e], acc[e]) : acc[e];
+  for (long long row = blockIdx.x * 4ll + (threadIdx.x >> 6); row < p.prows; row += gridDim.x * 4ll) {
+    PaRow w;
+    if (pt.by_row) {
+      w = {(int)(row / p.Hq / p.Lq), (int)(row / p.Hq % p.Lq), (int)(row % p.Hq)};
+    } else {
+      const int item = pt.whole + (int)(row / per), rb = item % pt.rowblocks, r = rb * per + (int)(row % per);
+      if (r >= pt.rows) continue;
+      w = pa_row(p.Lq, p.rep, pt.nper, item / pt.rowblocks / p.Hkv, item / pt.rowblocks % p.Hkv, r);
     }
-  }
-  T* o = reinterpret_cast<T*>(p.out) + w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2] + pa_channel<sizeof(T) == 2>(lane * E);
-  const float inv = total != 0.f ? 1.f / total : 0.f;
+    constexpr int E = D / 64, U = 8;
+    float m = PA_NONE, l = 0.f;                      // slots <= 64: one a lane
+    if (lane < p.slots) {
+      const float2 e = *reinterpret_cast<const float2*>(p.part_ml + (lane * p.prows + row) * 2);
+      m = e.x;
+      l = e.y;
+    }
+    float mj = m;
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
+    for (int o = 32; o > 0; o >>= 1) mj = fmaxf(mj, __shfl_xor(mj, o));
+    const float wt = l != 0.f ? __builtin_amdgcn_exp2f((m - mj) * p.sc2) : 0.f;
+    float total = l != 0.f ? l * wt : 0.f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const float* src = p.part_o + row * D + lane * E;
+    for (int s0 = 0; s0 < p.slots; s0 += U) {
+      float v[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u][e] = src[(long long)min(s0 + u, p.slots - 1) * p.prows * D + e];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int sl = min(s0 + u, 63);
+        const float ls = __shfl(l, sl), ws = __shfl(wt, sl);       // (lanes past the last slot: sum 0; a NaN sum is not 0 and stays)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = s0 + u < p.slots && ls != 0.f ? fmaf(ws, v[u][e], acc[e]) : acc[e];
+      }
+    }
+    T* o = reinterpret_cast<T*>(p.out) + w.b * p.os[0] + w.i * p.os[1] + w.h * p.os[2] + pa_channel<sizeof(T) == 2>(lane * E);
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
+  }
 }
 
 // ---- the plan of a call: which parts, which tile form, how many key splits.  A function of sizes and types alone (lengths stay on the device).
@@ -737,6 +737,7 @@ struct PaPlan {
 };
 
 constexpr int PA_SLOTS = 512;         // blocks that run at a time: two a CU
+constexpr long long PA_JOIN_ROWS = 1 << 24;      // rows a join launch has waves for (a grid has less than 2^32 threads); more take turns
 
 // two row tiles a wave where they leave two blocks a CU (fp32 heads of 128: 24 sequences of 413 queries over 77 + 622 keys 74 us with two, 50 with one)
 constexpr bool pa_two_row_tiles(int esz, int D) { return !(esz == 4 && D == 128); }
@@ -829,7 +830,7 @@ static void pa_launch(const PaPlan& plan, const PaParams& p, hipStream_t st) {
     }
   }
   if (plan.slots > 0)
-    hipLaunchKernelGGL((pa_join_kernel<T, D>), dim3((unsigned)((plan.prows + 3) / 4)), block, 0, st, p, 16 * plan.qt[0] * (plan.wk[0] ? 1 : 4));
+    hipLaunchKernelGGL((pa_join_kernel<T, D>), dim3((unsigned)(plan.prows < PA_JOIN_ROWS ? (plan.prows + 3) / 4 : PA_JOIN_ROWS / 4)), block, 0, st, p, 16 * plan.qt[0] * (plan.wk[0] ? 1 : 4));
 }
 
 }  // namespace pp

@@ -77,3 +77,24 @@ def test_scores_far_from_zero(hip, B, Lq, Hq, Hkv, D, P, S, size, dtype):
         four = mean(vs[:, lead]).mean(1, keepdim=True)
         lim = mean(vs[:, lead]).abs().mean(1, keepdim=True) * (80 * 2.0 ** -24 + (2.0 ** -11 if dtype == torch.float16 else 0)) + four.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25
         assert ((got - four).abs() <= lim).all()
+
+
+def test_more_rows_to_join_than_one_launch_has_waves(hip):
+    """2^26 rows, each the join of one prefix key and one suffix key"""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    B, Hq, D = 1 << 21, 32, 64
+    g = torch.Generator(device="cuda").manual_seed(9)
+    r = lambda *s: torch.randn(*s, D, generator=g, device="cuda", dtype=torch.float16)  # noqa: E731
+    q, pk, pv, k, v = r(B, 1, Hq), r(1, 1, 1), r(1, 1, 1), r(B, 1, 1), r(B, 1, 1)
+    out = torch.full_like(q, float("nan"))
+    hip.shared_prefix_attention(q, pk, pv, k, v, out=out)
+    for s in (slice(0, 2000), slice(B // 4 - 1000, B // 4 + 1000), slice(B // 2 - 1000, B // 2 + 1000), slice(B - 2000, B)):
+        q64, k64, v64 = (t[s].double() for t in (q, k, v))
+        d = ((q64 * k64).sum(-1) - (q64 * pk.double()).sum(-1)) * D ** -0.5
+        w = torch.sigmoid(d)[..., None]
+        want, size = w * v64 + (1 - w) * pv.double(), w * v64.abs() + (1 - w) * pv.double().abs()
+        scores = ((q64 * k64).abs().sum(-1) + (q64 * pk.double()).abs().sum(-1))[..., None] * D ** -0.5
+        lim = size * (2.0 ** -11 + 2.0 ** -24 * (2 * (D + 8) * scores + 70)) + want.abs() * 2.0 ** -11 + 2.0 ** -25
+        assert ((out[s].double() - want).abs() <= lim).all()
