@@ -446,7 +446,7 @@ int pp_ffn_fold_unfold(const void* in, void* out, int BT, int C, int H, int W, i
  * ---------------------------------------------------------------------------------------------- */
 /* GroupNorm + activation over an NHWC map (RAFT/extractor.py:14-18,123-124: norm_fn == 'group'): y = act((x - mean) / sqrt(var + eps) *
  * gamma + beta), mean / biased variance per image and group of C / groups consecutive channels, gamma / beta fp32 [C] or NULL (1 / 0).
- * in / out: channel windows [choff, choff + C) of NHWC buffers of dtype (out may be `in` itself, same window); C % 8 == 0, C <= 2048,
+ * in / out: channel windows [choff, choff + C) of NHWC buffers of dtype (out may be `in` itself, same window or one beside it); C % 8 == 0, C <= 2048,
  * groups divides C, strides and offsets multiples of 8, buffers 16-byte aligned.  act: any PP_ACT_* (slope of LRELU = act_param).
  * Channels of `out` outside its window are left as they are.  stats_ws: caller-owned fp32 workspace of
  * pp_group_norm_workspace_floats elements, 8-byte aligned (0 elements: NULL will do).  A NaN or infinity makes its group NaN.  Deterministic. */

@@ -801,24 +801,35 @@ def _raw_stream(who, x, *others):
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _refuse_overlap(who, out, *inputs):
-    """A given `out` may not share memory with what other blocks still read.  Views whose rows are the same stride apart may interleave
-    (columns of one buffer side by side)."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+class _Bytes:
+    """The addresses of a tensor's elements as numpy sees them (shape, strides; nothing is read through it)"""
+    def __init__(self, t):
+        n = t.element_size()
+        self.__array_interface__ = {"data": (t.data_ptr(), True), "shape": tuple(t.shape), "strides": tuple(n * s for s in t.stride()), "typestr": f"|V{n}", "version": 3}
 
+
+def _overlap(a, b):
+    """Do two tensors have a byte in common?  Exact, by shapes and strides: views of one buffer may lie side by side in any dimension (a pair of
+    views whose strides take numpy more than 10^5 steps to tell apart counts as overlapping)."""
+    if not a.numel() or not b.numel():
+        return False
+
+    def end(t):
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    if end(a) <= b.data_ptr() or end(b) <= a.data_ptr():
+        return False
+    try:
+        return np.shares_memory(np.asarray(_Bytes(a)), np.asarray(_Bytes(b)), max_work=100_000)
+    except np.exceptions.TooHardError:
+        return True
+
+
+def _refuse_overlap(who, out, *inputs):
+    """A given `out` may not share memory with what other blocks still read"""
     for t in inputs:
-        if t is None or not t.numel() or not out.numel():
-            continue
-        (a0, a1), (b0, b1) = span(out), span(t)
-        if a1 <= b0 or b1 <= a0:
-            continue
-        if out.dim() == 2 and t.dim() == 2:
-            pitch = out.stride(0) * out.element_size()
-            shift = (b0 - a0) % pitch if pitch else 0
-            if pitch == t.stride(0) * t.element_size() and out.shape[1] * out.element_size() <= shift and shift + t.shape[1] * t.element_size() <= pitch:
-                continue
-        raise ValueError(f"{who}: out overlaps an input")
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{who}: out overlaps an input")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -831,7 +842,7 @@ def _group_norm_floats(N, H, W, Cc, groups):
 
 def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, act_param=0.0, out=None, x_choff=0, C_=None, out_choff=0):
     """GroupNorm + activation over channels [x_choff, x_choff + C_) of x NHWC [N,H,W,Cx] -> channels [out_choff, ..) of `out` (allocated
-    [N,H,W,C_] if None; may be x itself with the same window).  gamma / beta fp32 [C_] or None; act: an ACT_* code (ACT_SILU included),
+    [N,H,W,C_] if None; may be x itself with the same window or one beside it).  gamma / beta fp32 [C_] or None; act: an ACT_* code (ACT_SILU included),
     act_param the slope of ACT_LRELU (pp_group_norm)."""
     require_gpu(x, "group_norm")
     N, H, W, Cx = x.shape
@@ -840,9 +851,9 @@ def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, act_par
         out = torch.empty((N, H, W, C_), dtype=x.dtype, device=x.device)
     else:
         assert out.is_contiguous() and out.dtype == x.dtype and out.shape[:3] == x.shape[:3]
-        if out.data_ptr() == x.data_ptr() and (out.shape != x.shape or out_choff != x_choff):
-            raise ValueError("group_norm: in place needs the same channel window")
-        _refuse_overlap("group_norm", out, x if out.data_ptr() != x.data_ptr() else None, gamma, beta)
+        if out.data_ptr() != x.data_ptr() or out.shape != x.shape or out_choff != x_choff:
+            _refuse_overlap("group_norm", out[..., out_choff:out_choff + C_], x[..., x_choff:x_choff + C_])
+        _refuse_overlap("group_norm", out[..., out_choff:out_choff + C_], gamma, beta)
     stream = _raw_stream("group_norm", x, gamma, beta, out)
     assert x.is_contiguous()
     assert gamma is None or (gamma.dtype == torch.float32 and gamma.is_contiguous() and gamma.shape == (C_,))
@@ -990,7 +1001,7 @@ def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal
     if out is None:
         out = torch.empty(qshape, dtype=dt, device=q.device)
     else:
-        _refuse_overlap("shared_prefix_attention", out, q, pk, pv, k, v, prefix_lens, lens)
+        _refuse_overlap("shared_prefix_attention", out, q, pk, pv, k, v, prefix_lens, lens)      # (slots of one buffer are no overlap)
     stream = _raw_stream("shared_prefix_attention", q, pk, pv, k, v, prefix_lens, lens, out)
     pshape, kshape = (G, P, Hkv, D), (B, S, Hkv, D)
     packed = []
