@@ -33,6 +33,11 @@ if os.environ.get("PP_DIAG") == "1":       # tuning builds: compiles the diagnos
     FLAGS.append("-DPP_DIAG")            # tools/bench_dcn.py select through pp_conv_args_t.impl (never in the shipped library)
 
 
+def flags(source):
+    """hipcc flags of one translation unit (a file name of csrc/); the tools that build variants of the library compile with the same"""
+    return FLAGS + FILE_FLAGS.get(source, [])
+
+
 def sources():
     """Every translation unit of the library (all of csrc/*.hip)."""
     return sorted(os.path.basename(p) for p in glob.glob(os.path.join(CSRC, "*.hip")))
@@ -101,7 +106,7 @@ def build(force=False, verbose=True):
                     for old in glob.glob(os.path.join(cache, f"{s[:-4]}.*.o")):
                         os.unlink(old)
                     obj_tmp = os.path.join(tmp, s.replace(".hip", ".o"))
-                    cmd = [hipcc] + FLAGS + FILE_FLAGS.get(s, []) + ["-c", os.path.join(CSRC, s), "-o", obj_tmp]
+                    cmd = [hipcc] + flags(s) + ["-c", os.path.join(CSRC, s), "-o", obj_tmp]
                     procs.append((s, obj_tmp, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
                 errors = []
                 for s, obj_tmp, obj, p in procs:

@@ -7,9 +7,9 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 NAME=$1; shift
 OUT=$R/build/$NAME
 mkdir -p $OUT
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
-/opt/rocm/bin/hipcc $F "$@" -c $R/propainter_amd/csrc/conv_gemm_v3.hip -o $OUT/conv_gemm_v3.o 2>/dev/null &
-/opt/rocm/bin/hipcc $F "$@" -c $R/propainter_amd/csrc/conv_gemm_v3s.hip -o $OUT/conv_gemm_v3s.o 2>/dev/null &
+library_flags() { python3 -c "import sys; sys.path.insert(0, '$R'); from propainter_amd import build; print(*build.flags('$1'))"; }
+/opt/rocm/bin/hipcc $(library_flags conv_gemm_v3.hip) "$@" -c $R/propainter_amd/csrc/conv_gemm_v3.hip -o $OUT/conv_gemm_v3.o 2>/dev/null &
+/opt/rocm/bin/hipcc $(library_flags conv_gemm_v3s.hip) "$@" -c $R/propainter_amd/csrc/conv_gemm_v3s.hip -o $OUT/conv_gemm_v3s.o 2>/dev/null &
 wait
 OTHERS=$(ls $R/propainter_amd/lib/obj/*.o | grep -v "conv_gemm_v3\.\|conv_gemm_v3s\.")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT/libpropainter_hip.so $OUT/conv_gemm_v3.o $OUT/conv_gemm_v3s.o $OTHERS

@@ -18,7 +18,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "propainter_amd", "csrc")
 OBJ = os.path.join(ROOT, "propainter_amd", "lib", "obj")
 HIPCC = "/opt/rocm/bin/hipcc"
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include")]
+sys.path.insert(0, ROOT)
+from propainter_amd import build          # noqa: E402
 TUS = sorted(os.path.basename(p)[:-4] for p in glob.glob(os.path.join(CSRC, "*.hip")))
 
 HELPER = '''// [variant build only] every launch asks for enough dynamic LDS that a block of an LDS-using kernel cannot share its CU with any other block
@@ -58,9 +59,9 @@ def exclusive_launches(text):
         depth, p, commas = 0, k, []
         while len(commas) < 4:
             c = text[p]
-            if c in "(<[":
+            if c in "([":             # (a kernel with template commas stands in parentheses; < and > are comparisons too)
                 depth += 1
-            elif c in ")>]":
+            elif c in ")]":
                 depth -= 1
             elif c == "," and depth == 0:
                 commas.append(p)
@@ -76,7 +77,7 @@ def exclusive_launches(text):
 
 def compile_all(src_dir, out_dir, names):
     os.makedirs(out_dir, exist_ok=True)
-    procs = [(b, subprocess.Popen([HIPCC] + FLAGS + ["-c", os.path.join(src_dir, b + ".hip"), "-o", os.path.join(out_dir, b + ".o")],
+    procs = [(b, subprocess.Popen([HIPCC] + build.flags(b + ".hip") + ["-I" + os.path.join(ROOT, "include"), "-c", os.path.join(src_dir, b + ".hip"), "-o", os.path.join(out_dir, b + ".o")],
                                   stdout=subprocess.DEVNULL, stderr=subprocess.PIPE)) for b in names]
     for b, pr in procs:
         err = pr.communicate()[1].decode()

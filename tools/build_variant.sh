@@ -6,10 +6,11 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 NAME=$1; shift
 OUT=$R/build/$NAME
 mkdir -p $OUT/obj
+library_flags() { python3 -c "import sys; sys.path.insert(0, '$R'); from propainter_amd import build; print(*build.flags('$1'))"; }
 pids=()
 for s in $R/propainter_amd/csrc/*.hip; do
   b=$(basename $s .hip)
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -DPP_DIAG "$@" -c $s -o $OUT/obj/$b.o &
+  /opt/rocm/bin/hipcc $(library_flags $b.hip) -DPP_DIAG "$@" -c $s -o $OUT/obj/$b.o &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait $p; done
