@@ -119,8 +119,8 @@ def parse(argv=None):
                     help="generator windows in flight on separate HIP streams (pipeline.InferenceConfig.window_streams)")
     ap.add_argument("--graph-lanes", action="store_true",
                     help="keep the window / RAFT lanes INSIDE the captured hipGraph (pipeline.ClipGraph(forked_branches=True)); default: the "
-                         "captured pass is one chain of launches -- with forked branches config 5 left wrong bytes in 3 of 64 replays "
-                         "(profiles/r6_c5_replays.txt); the lanes still serve eager submission")
+                         "captured pass is one chain of launches (the branches cost 23 GB of graph pool; until the convolutions waited for their "
+                         "LDS reads they left wrong bytes now and then: profiles/lds_read_wait.txt); the lanes still serve eager submission")
     ap.add_argument("--single-pass", action="store_true",
                     help="profiling aid: run exactly ONE eager pass of the clip and exit (what the rocprofv3 passes of "
                          "tools/gpu_profile.sh wrap, so that per-kernel counts are per pass)")

@@ -253,7 +253,8 @@ class _GenEngine:
                 # (round 6: a single window -- the clip's first / last windows, whose lengths differ from the rest -- is a group of ONE and
                 #  goes through the same path: its recurrent chain of ~100 small launches then runs on the pass's main stream in
                 #  ensure_propagated, never inside a window LANE.  Captured into a hipGraph, lanes carrying those chains gave ~5 % of the replays
-                #  a few hundred wrong bytes in one frame of exactly these windows -- profiles/r6_replay_bytes.txt; same arithmetic either way.)
+                #  a few hundred wrong bytes in one frame of exactly these windows -- profiles/r6_replay_bytes.txt -- until the convolutions' race on
+                #  their LDS stages was mended, profiles/lds_read_wait.txt; same arithmetic either way.)
                 if len(group) < 2 and os.environ.get("PP_CHAIN_IN_LANES") == "1":
                     continue                  # [diagnosis] rounds 2-5: a single window propagates inside its lane (the defect of profiles/r6_replay_bytes.txt)
                 gid = len(clip["prop_groups"])

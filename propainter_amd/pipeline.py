@@ -24,7 +24,7 @@ class InferenceConfig:
     fp16: bool = False
     batch_propagation: bool = True       # feature propagation of equal-length generator windows as one batch (InpaintGenerator.propagate_windows)
     # (both lane settings act on EAGER submission; a captured pass -- ClipGraph and the sharded graphs -- is one chain of launches unless
-    #  forked_branches=True: a forked hipGraph replayed wrongly a few per cent of the time at config 5, profiles/r6_c5_replays.txt)
+    #  forked_branches=True.  Lanes and branches left wrong bytes now and then until the convolutions waited for their LDS reads: profiles/lds_read_wait.txt)
     window_streams: int = 2      # engine extension: generator windows in flight on separate HIP streams (bit-identical results;
                                  # measured 1167.7 -> 1102.9 ms per 720p clip with 2, 1114.6 with 3: profiles/r2_window_streams.txt)
     raft_streams: int = 2        # engine extension: RAFT's two encoders, and its pair-directions in this many groups, on separate
@@ -332,11 +332,10 @@ class ClipGraph:
 
     def __init__(self, models, L, H, W, cfg: InferenceConfig, device, example=None, release_eager_pool=False, forked_branches=False):
         # forked_branches=False (default): the captured pass is ONE chain of launches -- no window lanes, no RAFT lanes.  Results are the
-        # same bytes either way (the lanes only reorder independent work), but on ROCm 7.2 a hipGraph with forked branches does not
-        # replay this pass reliably at every size: BASELINE config 5 (1080x1920x160, subvideo_length 20) with the 2 + 2 lanes left wrong
-        # bytes (max |d| 25) in 3 of 64 replays, the same graph without forked branches in 0 of 84; the 720x1280x80 pass with lanes
-        # 0 of ~250 (profiles/r6_c5_replays.txt).  The eager pass keeps cfg's lanes (30 eager passes with lanes: 0 deviations).
-        # forked_branches=True keeps cfg.window_streams / cfg.raft_streams inside the capture (-2 ... -3 % per pass): run self_check().
+        # same bytes either way (the lanes only reorder independent work).  The 1080x1920x160 pass (subvideo_length 20) with the 2 + 2 lanes in the
+        # graph left wrong bytes in 3 of 100 replays while the convolutions did not wait for their LDS reads ahead of a barrier, 0 of 100
+        # since (profiles/r6_c5_replays.txt, profiles/lds_read_wait.txt).
+        # forked_branches=True keeps cfg.window_streams / cfg.raft_streams inside the capture (-2 ... -3 % per pass, 23 GB more of graph pool).
         import dataclasses
         if not forked_branches:
             cfg = dataclasses.replace(cfg, window_streams=1, raft_streams=1)

@@ -791,13 +791,11 @@ class StreamingClipGraph:
     NSEG = 5          # compute segments of sharded_clip_steps: RAFT | completion | image propagation | windows | boundary blends
 
     def __init__(self, models, L, H, W, cfg, device, world=None, volume_gb=40.0, share_pool=True, single_graph=False, validate=8):
-        """DEFAULT (round 6): one graph per (rank, segment) in ONE memory pool, replayed chained in the wavefront order -- the form that
-        has never produced a wrong byte.  The overlapped form is opt-in because its failure mode is silent and unexplained: the
-        capture-time hazard checker (propainter_amd/hazard.py, tools/check_hazards.py) finds NO unordered access in the stage-pipelined
-        capture -- neither with the shipped stage map nor with flow completion on a third branch -- yet the third-branch map gives
-        frames that differ from the eager pass at 720x1280x320 (3 of 3 replays, profiles/r6_hazards.txt).  Whatever reorders those
-        bytes sits below the submitted program (runtime / cache coherence between concurrently running branches), so a validation on
-        the capture clip can only sample it.
+        """DEFAULT: one graph per (rank, segment) in ONE memory pool, replayed chained in the wavefront order.  The overlapped form is
+        opt-in: the capture-time hazard checker (propainter_amd/hazard.py, tools/check_hazards.py) finds no unordered access in the
+        stage-pipelined capture, yet it left wrong bytes (720x1280x320 with flow completion on a third branch: 3 of 3 replays,
+        profiles/r6_hazards.txt) until the convolutions waited for their LDS reads ahead of a barrier; 3 of 3 equal the eager pass since
+        (profiles/lds_read_wait.txt).
 
         single_graph=True (round 5): the whole wavefront as ONE hipGraph, pipelined by stage -- RAFT of the sub-videos on a
         branch forked from the capture stream (round 5 had image propagation on a second one: PP_SG_STAGES), flow completion, image
@@ -805,7 +803,7 @@ class StreamingClipGraph:
         (``_capture_single_graph``); ``validate`` replays of the captured graph are compared bit for bit with the eager pass at capture
         time, and a graph that does not reproduce it is replaced by the chained per-segment graphs (with a warning).  The overlap of the
         schedule lives INSIDE one graph (parallel branches: the form the whole-pass ClipGraph and the generator lanes use), not in
-        concurrent launches of several graphs, which give wrong frames on ROCm 7.2 (see ``replay``).  single_graph=False: one graph per
+        concurrent launches of several graphs (see ``replay``).  single_graph=False: one graph per
         (rank, segment), replayed chained (share_pool=True: one memory pool, capture order) or in the lockstep / concurrent A/B orders
         (share_pool=False)."""
         import dataclasses
@@ -816,7 +814,7 @@ class StreamingClipGraph:
             raise ValueError(f"a {L}-frame clip does not split into {self.world} sub-video blocks of {cfg.subvideo_length} frames")
         self.models, self.L, self.H, self.W = models, L, H, W
         # one RAFT lane per rank (the ranks run next to each other) and no window lanes: no forked branches inside a captured graph beyond
-        # the stage map's own (pipeline.ClipGraph: config 5 with lanes left wrong bytes in 3 of 64 replays, without in 0 of 84)
+        # the stage map's own (as pipeline.ClipGraph)
         self.cfg = dataclasses.replace(cfg, raft_streams=1, window_streams=1)
         self.volume_gb = float(volume_gb)
         self.single_graph = bool(single_graph)
@@ -961,15 +959,10 @@ class StreamingClipGraph:
         try:
             with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                 cur = torch.cuda.current_stream(dev)
-                # which stages leave the capture stream: RAFT (0) and image propagation (2) on branches of their own, flow completion (1)
-                # with the windows on the capture stream.  MEASURED at BASELINE config 4 (720x1280x320, profiles/r5_streaming_single_graph.txt):
-                # with flow completion on a third branch the LAST sub-video's completed flows differed from replay to replay (max 0.025 px,
-                # +-1 byte in 0.2 % of that sub-video's bytes; smaller clips never showed it, the kernels are bit-stable next to unrelated
-                # load, lanes on / off made no difference); with this map every stage of every rank equals the eager pass and the pass is
-                # 2 % faster (flow completion is latency-bound and overlaps the windows' tail either way).  PP_SG_STAGES overrides (diagnosis).
-                # Round 6 (profiles/r6_replay_bytes.txt): what goes wrong on a forked branch is a long chain of small dependent launches -- flow
-                # completion here, a window's feature propagation in the whole-pass graph (~5 % of its replays until round 6).  Image
-                # propagation (158 steps of 20 us) is such a chain too, so the default map keeps only RAFT's large launches on a branch.
+                # which stages leave the capture stream: RAFT (0) alone.  Flow completion on a branch of its own gave flows that differed from
+                # replay to replay at 720x1280x320 (profiles/r5_streaming_single_graph.txt) while the convolutions had a race on their LDS stages
+                # (profiles/lds_read_wait.txt); without that map the pass is 2 % faster (flow completion is latency-bound and overlaps the windows'
+                # tail either way).  PP_SG_STAGES overrides.
                 on_side = {int(v) for v in os.environ.get("PP_SG_STAGES", "0").split(",") if v != ""}
                 # PP_SG_FENCE (diagnosis, round 6; bit 0: L2 write-back kernel in front of every segment's event, bit 1: L2 invalidate kernel
                 # behind every cross-branch wait): tests whether the deviation of the three-branch map is a cache-visibility defect of
@@ -1037,16 +1030,10 @@ class StreamingClipGraph:
         run_logical_shards_graphed: the A/B reference of the streaming order).
 
         concurrent (default: env PP_STREAM_CONCURRENT == "1", else False; single_graph=False only): let the ranks' segment graphs
-        overlap on their streams, ordered by the exchange events only.  UNSAFE on ROCm 7.2 / MI355X, kept for diagnosis: 10-14 of 16
-        passes give wrong frames (tools/diag_stream2.py, profiles/r5_streaming_single_graph.txt).  Round 5 narrowed it down: it is a race
-        between graph launches that are in flight at the same time, not stale input -- a second pass over the same inputs is wrong as
-        often (round 4 read "never" off a luckier box); it does not need the copy engine (inputs written by a device kernel: same rate),
-        shared module state (private engines per rank: same), forked branches inside the graphs (window_streams=1: same), memcpy
-        exchanges (kernel copies: same) nor a runtime flag (DEBUG_CLR_GRAPH_PACKET_CAPTURE=0, GPU_MAX_HW_QUEUES=8,
-        HIP_FORCE_DEV_KERNARG=0: same); the kernels themselves are bit-exact next to unrelated load (tools/diag_noise.py) and on a
-        forked branch of one graph (tools/diag_branch.py).  The overlapped schedule therefore ships as ONE graph
-        (``single_graph=True``: 0 wrong first passes of 24, 17 % faster than the chained launches at the diagnostic size); this
-        multi-graph form stays chained by default (wavefront issue order, no overlap) and warns when the overlap is requested."""
+        overlap on their streams, ordered by the exchange events only.  10-14 of 16 passes gave wrong frames (tools/diag_stream2.py,
+        profiles/r5_streaming_single_graph.txt) while the convolutions did not wait for their LDS reads ahead of a barrier; 0 of 16 since
+        (34x128x192, profiles/lds_read_wait.txt).  No larger clip has been run since, so this form stays chained by default (wavefront issue order,
+        no overlap) and warns when the overlap is requested; ``single_graph=True`` is the overlapped schedule as ONE graph."""
         if concurrent is None:
             concurrent = os.environ.get("PP_STREAM_CONCURRENT") == "1"
         if self.order is None:
@@ -1058,9 +1045,8 @@ class StreamingClipGraph:
             return self._single_out.clone()               # a fresh tensor like the chained form's: the next replay overwrites the static buffer
         if concurrent:
             import warnings
-            warnings.warn("StreamingClipGraph.replay(concurrent=True): overlapping launches of several hipGraphs give WRONG frames in most "
-                          "passes on ROCm 7.2 / MI355X (profiles/r5_streaming_single_graph.txt); use single_graph=True for the overlapped "
-                          "schedule", RuntimeWarning, stacklevel=2)
+            warnings.warn("StreamingClipGraph.replay(concurrent=True): overlapping launches of several hipGraphs are checked at 34x128x192 alone "
+                          "(profiles/lds_read_wait.txt); use single_graph=True for the overlapped schedule", RuntimeWarning, stacklevel=2)
         if self.share_pool and (lockstep or concurrent):
             raise ValueError("StreamingClipGraph(share_pool=True): the graphs share one memory pool and must replay in their capture "
                              "order, one after the other; build with share_pool=False for the lockstep / concurrent orders")
