@@ -486,7 +486,8 @@ int pp_linear_i8_tokens(const void* x, int64_t x_rstride, int x_dtype, const voi
  * prompt.  Query head h reads key head h / (Hq / Hkv).  Of the prefix the first prefix_lens[g] of P keys count, of the suffix the first
  * lens[b] of S (values are clamped to [0, P] / [0, S]; what lies behind them is never used, NaN included); with causal = 1 query i sees
  * suffix keys up to lens[b] - Lq + i (the queries are the last Lq tokens of the sequence), and the values hidden from it have to be finite.  A
- * query without keys gives zeros.  out may not overlap an input.
+ * query without keys gives zeros.  out may not overlap an input.  fp16: the softmax weights are rounded to fp16 as the second product's operand (lifted by
+ * 2^15, so weights down to 2^-39 of the largest count); scores, sums and outputs are held in fp32 until the outputs are rounded.
  * Strides in elements, multiples of 8 (fp16) / 4 (fp32), the last dimension (D) contiguous, buffers 16-byte aligned; token strides >= D. */
 typedef struct {
   int32_t dtype;                        /* PP_F16 / PP_F32: q, keys, values, out                   */

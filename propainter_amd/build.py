@@ -23,7 +23,9 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpropainter_hip.so")
 STAMP_PATH = os.path.join(LIB_DIR, "build_stamp.txt")
 # packed-fp32-ops off: hipcc otherwise turns ordinary float code into v_pk_{add,mul,fma}_f32, some forms of which have given wrong results
-# now and then; the scalar instructions round alike, so results are unchanged (the host pass warns that it does not know the feature)
+# now and then (the host pass warns that it does not know the feature).  The scalar instructions round alike, but hipcc merges other pairs of a product and a
+# conversion to fp16 without the packed ones: a quarter of the fp16 window attention's outputs, rounded once before, are rounded twice, and the fp16
+# generator's bytes moved by one in 0.8 % of the values (8 frames of 240x432).
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # These round a product to fp32 before they round it to fp16, as they did while their products were packed: without the packed instructions hipcc

@@ -5,8 +5,9 @@
 //
 // Statistics are held in fp32 as (count, mean, sum of squared deviations) and joined pairwise (Chan et al. 1979): no difference of large
 // sums of squares, so a map whose mean is far from zero loses nothing.  The order of every sum is fixed by the sizes: no atomics.
-// Bound by memory: the map is read twice (the second time partly from the cache) and written once, 4x360x640x64 fp16 in 75 us = 4.7 TB/s of
-// those three passes.
+// Bound by memory: the map is read twice (the second time partly from the cache) and written once, 4x360x640x64 fp16 in 75 us (kernels 25 + 43) =
+// 4.7 TB/s of those three passes.  Every output block joins all slices of all groups of its image first, which counts where groups are many and images
+// few: 1x540x960x64 fp16 in 8 / 32 / 64 groups 58 / 115 / 190 us.
 #include "common.h"
 #include "attn_lanes.h"
 #include <type_traits>
@@ -55,7 +56,7 @@ __device__ __forceinline__ void join_parts(int per, int ng, int s0, float& cnt, 
 // squared deviations are taken in two passes, and joined to what the thread has.  Values are taken relative to the slice's first pixel (per
 // channel), so that means hold deviations and not magnitudes; it may itself lie far from the rest (a border of zeros): nothing is subtracted
 // from sums of squares.
-constexpr int GN_U = 8;
+constexpr int GN_U = 8;        // (2, 4 and 8 pixels: 23.9 / 25.4 / 25.4 us at 4x360x640x64 fp16, 19.0 / 18.8 / 19.4 at 2x270x480x96 fp32; most merges are saved by 8)
 template <typename T>
 __global__ __launch_bounds__(256) void gn_stats_kernel(const GnParams p) {
   __shared__ float s1[256 * 8], s2[256 * 8], parts[3][256];
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnParams p) {
   const T* x = reinterpret_cast<const T*>(p.in) + (long long)n * p.HW * p.in_cs + p.in_co + col * 8;
   T* y = reinterpret_cast<T*>(p.out) + (long long)n * p.HW * p.out_cs + p.out_co + col * 8;
   const long long q0 = (long long)blockIdx.x * p.ppblock, q1 = min(q0 + p.ppblock, (long long)p.HW);
-  constexpr int U = 2;                                  // loads in flight a thread (at 4x360x640x64 fp16 / 2x270x480x96 fp32: 1: 77.5 / 66.6 us, 2: 78.5 / 66.0, 4: 86.4 / 69.9)
+  constexpr int U = 2;                                  // loads in flight a thread (at 4x360x640x64 fp16 / 2x270x480x96 fp32: 1 or 2 are the same within noise, 77.5 / 66.6 and 78.5 / 66.0 us in one run; 4: 86.4 / 69.9)
   for (long long q = q0 + pr; q < q1; q += U * rows) {
     float v[U][8];
 #pragma unroll

@@ -406,7 +406,7 @@ __global__ __launch_bounds__(512) void lin_i8_thin_kernel(const LinI8Params p) {
 // Small calls on float tokens: a block takes up to 16 tokens (2048 vectors of 8 in all) and 16 channels and makes the tokens' codes itself, into LDS --
 // they come out of L2, and a launch and a round trip of the codes are saved.  Replayed / called (us): 45 x 512 -> 1536 5.7 / 9 against 6.5 / 14.4 with
 // two launches, 200 x 512 -> 512 6.6 / 9 against 7.4 / 14.6; with more blocks every one of them quantises too much: 400 x 512 -> 512 (800 blocks)
-// 9.3 against 7.6 replayed.  One token is always taken here.
+// 9.3 against 7.6 replayed.  One token is taken here up to K = 16384 (1 x 4096 -> 4096: 6.6 us kernel time, 11 a call).
 constexpr int I8_FUSE_VEC = 4;                     // vectors a thread
 constexpr int64_t I8_FUSE_BLOCKS = 512;            // two a CU
 inline int i8_fused_rows(int64_t M, int N, int K) {  // tokens a block (0: two launches)
@@ -476,8 +476,8 @@ __global__ __launch_bounds__(512) void lin_i8_token_kernel(const LinI8Params p, 
 // passing registers (16 bytes a lane, one kilobyte an instruction), S stages of 64 k deep: the weights' kilobytes are in operand order
 // already, the lanes of a token piece gather 16 rows x 4 pieces so that it lands in operand order too -- fragment reads are then
 // lane-linear and free of bank conflicts without any swizzle.  Token rows past M repeat the last one, channel blocks past N the last one.
-// Bound by the matrix cores: 8192^3 470-500 us = 2.2-2.3 POP/s (all fragment reads of a stage ahead of its products; in the compiler's order
-// 597), MFMA busy 48-51 % at 2.0 GHz, the share that a large fp16 product of the vendor library reaches too.  LDS is not what holds it: 4 waves of
+// Bound by the matrix cores: 8192^3 488-494 us = 2.2 POP/s on a card that has been busy, 576 in the first calls on an idle one (the vendor library's
+// product beside it 438-446; all fragment reads of a stage ahead of its products; in the compiler's order 597).  LDS is not what holds it: 4 waves of
 // 128 x 128 with the next stage's operands read during this one's products, half the LDS bytes a product and no wait among them, took 511
 // against 496, and weights from the cache straight into registers 665.
 typedef __attribute__((address_space(3))) void* i8_lptr;
@@ -584,8 +584,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_i8_tile_kernel(const Li
 
 // Short K, many tokens: the output's bytes are the work.  A block of 4 waves keeps the weights of 256 channels in registers (64 a wave, KT operand
 // tiles deep) for the whole launch and streams token tiles of 64 through two LDS stages.  The `panels` blocks that read the same tokens
-// run next to each other on one XCD (block id mod 8).  Bound by the stores: 110160 x 512 -> 1536 in fp16 110-118 us for 338 MB of output
-// and 56 MB of codes (3.5 TB/s).  With the quantiser, 137: stores past the cache 149 against 147 then, outputs held back a tile 148 against 133 then.
+// run next to each other on one XCD (block id mod 8).  Bound by the stores: 110160 x 512 -> 1536 in fp16 119 us (112 at best) for 338 MB of output
+// and 56 MB of codes (3.3 TB/s).  With the quantiser, 137: stores past the cache 149 against 147 then, outputs held back a tile 148 against 133 then.
 template <typename TO, int KT>
 __global__ __launch_bounds__(256, 2) void lin_i8_stream_kernel(const LinI8Params p, const int panels, const int groups, const int tiles) {
 #if defined(__HIP_DEVICE_COMPILE__)

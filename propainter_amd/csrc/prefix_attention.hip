@@ -10,16 +10,18 @@
 // pa_join_kernel joins them in a fixed order.
 //
 // S^T = K Q^T and O^T += V^T P^T on 16x16 MFMA tiles: a lane holds scores of ONE query (column l & 15), so the row maximum takes two lane
-// swaps, and its scores are the second product's operand as they are, keys relabelled.  Maximum, sum and output stay in fp32 registers;
-// fp16 weights are rounded once, to the values' type.
+// swaps, and its scores are the second product's operand as they are, keys relabelled.  Maximum, sum and output stay in fp32 registers.
+// fp16 calls round every weight once to fp16: the matrix instructions take both operands in one type, and weights in two fp16 parts would double the second
+// product.  It costs 2^-11 of a weight at most; over the shapes below the error against 64 bits is 2.4e-4 to 2.6e-4 of the outputs' size, 2.1e-4 of
+// which is the rounding of the outputs themselves.
 //
 // Forms (4 waves a block).  Many rows: a wave owns 16 QT rows and every key of a tile of 64 that lies in LDS (K and V swizzled, fp32 V
 // skewed), the next tile's loads in flight during the products.  Few rows (WK): the four waves share 16 QT rows and take different keys,
 // joined through LDS at the end; in fp16 every wave streams keys of its own (pa_stream_block).
-//   rows: 24 sequences x 765 queries, 4 heads of 128, 2430 shared + 1158 own keys, fp16: 181 us = 750 TFLOP/s.  Products alone would be 117 us at the rate
-//     of a large matrix product; the softmax' vector instructions take 190 of 407 thousand cycles a CU next to 130 of MFMA, and two blocks a
+//   rows: 24 sequences x 765 queries, 4 heads of 128, 2430 shared + 1158 own keys, fp16: 181 us = 750 TFLOP/s (181 and a join of 10 under the profiler).  Products alone would be 102 us at the
+//     rate of a large matrix product; the softmax' vector instructions take 190 of 407 thousand cycles a CU next to 130 of MFMA, and two blocks a
 //     CU overlap them in part.  LDS conflicts: none.  Two LDS tiles (one barrier a tile, one block a CU): 193.
-//   single tokens: 64 sequences, 8192 shared + up to 1024 own keys, 32 heads on 8 key heads of 128, fp16: 55 us for 171 MB; the two parts run in one launch
+//   single tokens: 64 sequences, 8192 shared + up to 1024 own keys, 32 heads on 8 key heads of 128, fp16: 54-59 us for 171 MB (68.7 with every suffix full, 48.9 half full); the two parts run in one launch
 //     (44 us: the suffixes out of memory next to the packed rows' products), 6 us of joining, the rest launches.
 //   fp32: 16 sequences x 4 queries, 16 heads on 2 key heads of 64, 4096 + up to 512 keys: 26 us, of which 6.6 are products at the fp32 matrix
 //     rate; few waves, so the latency of a tile's loads and dependent products, and the join's 6 us.
@@ -782,7 +784,7 @@ inline PaPlan pa_plan(const pp_prefix_attn_args_t* a) {
   if (packed && a->S > 0) {
     add(1, 0, 1, PA_SLOTS, true);
     // Blocks for the packed rows: every split leaves outputs to join, and their blocks take the place of suffix walks, so no more than finish their
-    // products while the suffixes (taken as half full) come out of memory, and at most one a CU.  A tile's products take about 2 us (two fp16
+    // products while the suffixes (taken as half full: the plan knows sizes, the lengths stay on the device) come out of memory, and at most one a CU.  A tile's products take about 2 us (two fp16
     // row tiles of 16; fp32 four times that), the suffixes come at 4.3 TB/s.  Against 256 always (us): 64 sequences behind 8192 keys, suffixes up to
     // 1024: 54 / 64.5, behind 2048: 46 / 50; 16 sequences behind 32768 keys, suffixes up to 512, where 128 blocks are too few: 50 with 256, 71.5.
     const long long prows = R * nseq;

@@ -990,7 +990,8 @@ def shared_prefix_attention(q, pk, pv, k, v, prefix_lens=None, lens=None, causal
     q [B,Lq,Hq,D]; pk / pv [G,P,Hkv,D] or None; k / v [B,S,Hkv,D] or None; Hq a multiple of Hkv, D 64 or 128, fp16 or fp32, any strides with a
     contiguous last dimension.  Sequence b belongs to group b // (B // G).  prefix_lens int32 [G] / lens int32 [B] (device): the keys that
     count (default: all); causal: query i sees suffix keys up to lens[b] - Lq + i, and the values that causality hides from a query have to
-    be finite.  scale: default 1 / sqrt(D).  A query without keys gives zeros.  A given `out` may not overlap an input.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
+    be finite.  scale: default 1 / sqrt(D).  A query without keys gives zeros.  A given `out` may not overlap an input (slots of one
+    buffer do not).  fp16: the weights are rounded once to fp16, everything else is fp32 up to the output.  Returns [B,Lq,Hq,D] (pp_shared_prefix_attention)."""
     require_gpu(q, "shared_prefix_attention")
     B, Lq, Hq, D = qshape = q.shape
     dt = q.dtype
